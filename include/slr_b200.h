@@ -87,8 +87,10 @@ SLR_API const char* slr_last_error(void);
  * process-wide, e.g. to leave SMs to NCCL kernels that run alongside in a
  * multi-GPU step.  No reference counterpart. */
 SLR_API int slr_set_sm_limit(int n);
-/* Reads and clears the device-side status word that bounded waits set when
- * they time out (SLR_OK or SLR_ERR_TIMEOUT).  Synchronises the device. */
+/* Reads and clears the device-side status words: SLR_ERR_TIMEOUT when a
+ * bounded wait gave up, else SLR_ERR_BAD_INDEX when a kernel of the paged
+ * cache or slr_token_logprobs met an index out of range (and left it out),
+ * else SLR_OK.  Synchronises the device. */
 SLR_API int slr_device_status(int* status_out);
 
 /* ------------------------------------------------- in-place BSR addmm -- */
@@ -404,6 +406,144 @@ SLR_API size_t slr_nm_linear_workspace_size(const slr_nm_layer* layer, int64_t M
  */
 SLR_API int slr_nm_linear_forward(const slr_nm_layer* layer, const void* x, int64_t ldx, void* y, int64_t ldy,
                                   int64_t M, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------ paged K/V cache -- */
+
+/*
+ * Keys and values of up to max_rows sequences ("rows") in pages of page_size
+ * tokens, all layers in one pool, with the book-keeping on the device so that
+ * no call waits for the host (every call can be captured into a graph).  The
+ * reference keeps no cache: it recomputes the prefix every step
+ * (ssalaad/inference/generate.py:12-26).
+ *
+ * Token t of row b lies in page table[b][t / page_size], slot t % page_size.
+ * Layer i's K of page p, key head h, slot s starts at
+ *   k + i * layer_stride + p * page_stride + h * head_stride + s * token_stride
+ * (elements, head_dim of them contiguous), V likewise from v.  The block of
+ * one page (kv_heads x page_size x head_dim) is contiguous in memory, in
+ * either order of heads and slots.
+ *
+ * state: device int32, SLR_KV_HEADER_WORDS + max_rows + num_pages +
+ * max_rows * max_pages words:
+ *   header  [0] pages that were missing in the last slr_kv_advance
+ *           [1] rows that would have outgrown max_pages in it
+ *           [2] pages copied or moved by the last _advance / _compact
+ *           [3] pages in use
+ *   lens    [max_rows] tokens of each row (0 = empty)
+ *   refs    [num_pages] table entries that name the page (0 = free)
+ *   table   [max_rows][max_pages], -1 where a row has no page
+ * An empty cache is a header, lens and refs of zeros and a table of -1.
+ *
+ * Kernels check every page number, length and row they read; what is out of
+ * range is left out and reported as SLR_ERR_BAD_INDEX by slr_device_status.
+ *
+ * Limits: head_dim a multiple of 8 up to 256; page_size a multiple of 16 up
+ * to 1024; strides multiples of 16 bytes, k and v 16-byte aligned; max_rows
+ * up to SLR_KV_MAX_ROWS; max_pages * page_size below 2^31.
+ */
+#define SLR_KV_HEADER_WORDS 4
+#define SLR_KV_MAX_ROWS 2048
+
+typedef struct slr_kv_cache {
+  void* k;                /* device, dtype: layer 0's K pages */
+  void* v;                /* device, dtype: layer 0's V pages */
+  int32_t* state;         /* device int32, as above */
+  int64_t layer_stride;   /* elements from a layer's K (V) to the next's */
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t token_stride;
+  int32_t num_layers;
+  int32_t num_pages;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t max_rows;
+  int32_t max_pages;      /* pages a row can hold */
+  int32_t dtype;          /* slr_dtype */
+} slr_kv_cache;
+
+/* Device bytes of scratch for slr_kv_advance and slr_kv_compact / for
+ * slr_kv_attend with any number of rows up to max_rows (0 on a bad
+ * descriptor).  256-byte aligned, not shared by calls that may overlap on
+ * the GPU, needs no initialisation and keeps nothing between calls. */
+SLR_API size_t slr_kv_pages_workspace_size(const slr_kv_cache* cache);
+SLR_API size_t slr_kv_attend_workspace_size(const slr_kv_cache* cache);
+
+/*
+ * The book-keeping of one step, for all rows at once:
+ *   1. Row i becomes a copy of row parents[i] as it was before the call
+ *      (parents[i] < 0: empty); parents NULL keeps every row.  Rows with the
+ *      same parent share its pages (fork); pages that no row names any more
+ *      are free.
+ *   2. Row i changes its length by n_new[i]; with n_new NULL, every row that
+ *      holds tokens does so by n_all.  A negative change drops tokens from the
+ *      end (not below 0) and frees pages.  A positive one gives the row new
+ *      pages, the lowest free numbers in row order; a row whose last page is
+ *      partly filled and shared gets its own copy of that page first (of
+ *      all layers), unless every sharer grows and it is the lowest of them.
+ * Growth is all or nothing: when pages are missing or a row would outgrow
+ * max_pages, no row grows and header words 0 and 1 say by how much.
+ * parents, n_new: device int32 [max_rows].
+ */
+SLR_API int slr_kv_advance(const slr_kv_cache* cache, const int32_t* parents, const int32_t* n_new,
+                           int32_t n_all, void* workspace, size_t workspace_bytes, void* stream);
+/* Moves the live pages to the numbers below their count (header word 3): the
+ * live pages at or above it go, in ascending order, to the free ones below,
+ * and the table is rewritten.  Pages from header word 3 on are free after it. */
+SLR_API int slr_kv_compact(const slr_kv_cache* cache, void* workspace, size_t workspace_bytes, void* stream);
+/* Copies pages src[i] -> dst[i] of every layer, i < n (device int32), as
+ * bytes; the state is not touched.  A pair whose number is out of range, whose
+ * dst is another pair's src or dst, or whose src is another's dst is left out
+ * and reported (SLR_ERR_BAD_INDEX). */
+SLR_API int slr_kv_copy_pages(const slr_kv_cache* cache, const int32_t* src, const int32_t* dst, int32_t n,
+                              void* stream);
+/*
+ * Writes new tokens' K and V [tokens, kv_heads, head_dim] (row and head
+ * strides in elements, head_dim contiguous) into `layer`, after slr_kv_advance
+ * has made room: the n_b tokens of row b go to its last n_b positions.
+ * cu_tokens: device int32 [max_rows + 1], row b's tokens are [cu[b], cu[b+1]);
+ * tokens from cu[max_rows] on are ignored.  NULL: token i is row i's (tokens
+ * <= max_rows), rows of length 0 are skipped.
+ */
+SLR_API int slr_kv_append(const slr_kv_cache* cache, int32_t layer, const void* k, int64_t k_row_stride,
+                          int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                          int64_t tokens, const int32_t* cu_tokens, void* stream);
+/*
+ * Attention of one token per row, rows 0 .. rows-1 of the cache:
+ * out[b, h] = softmax(scale * q[b, h] . K_t) . V_t over the tokens t < lens[b]
+ * of `layer` at key head h / (heads / kv_heads).  q and out [rows, heads,
+ * head_dim] with row and head strides in elements; lse (NULL, or float32
+ * [rows, heads]) receives the log of the sum of exponentials.  A row of length
+ * 0, or whose scores are all -inf, gives zeros and lse = -inf; a NaN or +inf
+ * score gives NaN.  Slots behind a row's length are never read into the
+ * result, whatever they hold.  Products and sums are fp32; the
+ * probabilities are kept to at least 16 bits; out is rounded once.  The
+ * result does not depend on timing, only on lens and the GPU's SM count.
+ */
+SLR_API int slr_kv_attend(const slr_kv_cache* cache, int32_t layer, const void* q, int64_t q_row_stride,
+                          int64_t q_head_stride, void* out, int64_t o_row_stride, int64_t o_head_stride,
+                          float* lse, int32_t rows, int32_t heads, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------- scores of tokens -- */
+
+#define SLR_MAX_TOP 32
+/*
+ * Log probabilities under softmax(logits[i]) for logits [rows, vocab] (dtype,
+ * rows row_stride elements apart, 0 = vocab; any alignment of the element):
+ *   logprob [rows]       of targets[i]; 0 where targets[i] < 0; NaN and
+ *                        SLR_ERR_BAD_INDEX (slr_device_status) from vocab on
+ *   entropy [rows]       -sum p log p, with 0 log 0 = 0
+ *   top_ids, top_logprobs [rows, top]  the best tokens, greatest first, equal
+ *                        values by lower index (-0 = +0, NaN as -inf)
+ * all float32 (top_ids int64).  targets with logprob, entropy, and the top
+ * pair (top = 0 .. SLR_MAX_TOP, at most vocab) may each be NULL.  A row that
+ * holds a NaN or +inf, or nothing but -inf, gives NaN (not for targets[i] <
+ * 0), as log_softmax does; other -inf logits are tokens of probability 0.
+ */
+SLR_API int slr_token_logprobs(const void* logits, int64_t row_stride, int64_t rows, int64_t vocab, int dtype,
+                               const int64_t* targets, float* logprob, float* entropy, int32_t top,
+                               int64_t* top_ids, float* top_logprobs, void* stream);
 
 /* --------------------------------------------------- dense -> BSR -- */
 

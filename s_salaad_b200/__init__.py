@@ -6,9 +6,11 @@ The package mirrors the reference's module and operator API
 (``efficient.LRSLinear``, ``efficient.dense_to_bsr``,
 ``efficient.build_efficient_model``, ``cuda_sparse.register_reference_op``);
 ``ops.LayerGroup`` runs layers that read one input together and ``shard``
-splits a layer by block-rows over several GPUs.  CUDA only; no CPU fallback.
+splits a layer by block-rows over several GPUs.  ``kvcache.PagedCache`` and
+``ops.token_logprobs`` are the operators around those layers that serving a
+model needs.  CUDA only; no CPU fallback.
 """
-from . import ops
+from . import kvcache, ops
 from ._lib import LIB_PATH, load
 
-__all__ = ["ops", "load", "LIB_PATH"]
+__all__ = ["kvcache", "ops", "load", "LIB_PATH"]

@@ -71,6 +71,14 @@ EXPORTED = (
     "slr_nm_compress",
     "slr_nm_linear_workspace_size",
     "slr_nm_linear_forward",
+    "slr_kv_pages_workspace_size",
+    "slr_kv_attend_workspace_size",
+    "slr_kv_advance",
+    "slr_kv_compact",
+    "slr_kv_copy_pages",
+    "slr_kv_append",
+    "slr_kv_attend",
+    "slr_token_logprobs",
 )
 
 SLR_MAX_RANKS = 8
@@ -78,6 +86,9 @@ SLR_IPC_HANDLE_BYTES = 64
 SLR_SIGNAL_WORDS = 32
 SLR_DECODE_CTRL_BYTES = 4096
 SLR_DECODE_MAX_TOKENS = 32
+SLR_KV_HEADER_WORDS = 4
+SLR_KV_MAX_ROWS = 2048
+SLR_MAX_TOP = 32
 
 i64, i32, vp, sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
 
@@ -121,6 +132,28 @@ class SlrNmLayer(ctypes.Structure):
         ("bias", ctypes.c_void_p),
         ("dtype", ctypes.c_int32),
         ("flags", ctypes.c_int32),
+    ]
+
+
+class SlrKvCache(ctypes.Structure):
+    """Mirror of ``struct slr_kv_cache``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("state", ctypes.c_void_p),
+        ("layer_stride", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("num_layers", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
     ]
 
 
@@ -188,6 +221,15 @@ _SIGS = {
     "slr_nm_compress": ([vp, i64, i64, i32, vp, vp, vp], i32),
     "slr_nm_linear_workspace_size": ([ctypes.POINTER(SlrNmLayer), i64], sz),
     "slr_nm_linear_forward": ([ctypes.POINTER(SlrNmLayer), vp, i64, vp, i64, i64, vp, sz, vp], i32),
+    "slr_kv_pages_workspace_size": ([ctypes.POINTER(SlrKvCache)], sz),
+    "slr_kv_attend_workspace_size": ([ctypes.POINTER(SlrKvCache)], sz),
+    "slr_kv_advance": ([ctypes.POINTER(SlrKvCache), vp, vp, ctypes.c_int32, vp, sz, vp], i32),
+    "slr_kv_compact": ([ctypes.POINTER(SlrKvCache), vp, sz, vp], i32),
+    "slr_kv_copy_pages": ([ctypes.POINTER(SlrKvCache), vp, vp, ctypes.c_int32, vp], i32),
+    "slr_kv_append": ([ctypes.POINTER(SlrKvCache), ctypes.c_int32, vp, i64, i64, vp, i64, i64, i64, vp, vp], i32),
+    "slr_kv_attend": ([ctypes.POINTER(SlrKvCache), ctypes.c_int32, vp, i64, i64, vp, i64, i64, vp, ctypes.c_int32,
+                       ctypes.c_int32, ctypes.c_float, vp, sz, vp], i32),
+    "slr_token_logprobs": ([vp, i64, i64, i64, i32, vp, vp, vp, ctypes.c_int32, vp, vp, vp], i32),
 }
 
 _lock = threading.Lock()

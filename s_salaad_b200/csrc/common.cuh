@@ -37,6 +37,9 @@ int cuda_fail(cudaError_t e, const char* what);
 // Device status word (one per translation unit that waits on the device);
 // a bounded wait that gives up ORs SLR_TIMEOUT_BIT into it.
 constexpr unsigned SLR_TIMEOUT_BIT = 1u;
+// A kernel of the paged cache or of the token scores met an index out of range
+// (a page, a length, a row, a token) and left it out.
+constexpr unsigned SLR_BAD_INDEX_BIT = 2u;
 // 2 s of %globaltimer: far above any legitimate wait inside one launch.
 constexpr unsigned long long SLR_WAIT_LIMIT_NS = 2000000000ull;
 

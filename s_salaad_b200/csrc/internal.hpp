@@ -199,6 +199,78 @@ int launch_validate_bsr(const int32_t* crow, int64_t NB, const int32_t* col, int
                         int64_t nbk, const int32_t* active, int64_t active_nb, int* flag,
                         cudaStream_t s);
 
+// ---- paged key-value cache (k_attend.cu, k_pages.cu).  Strides in elements.
+constexpr int kAttendMaxRows = SLR_KV_MAX_ROWS;  // rows of a cache: their lengths are kept in shared memory
+struct AttendArgs {
+  const void* k = nullptr;  // first page of the layer
+  const void* v = nullptr;
+  int64_t page_stride = 0, head_stride = 0, token_stride = 0;
+  const int32_t* table = nullptr;  // [rows, max_pages]
+  const int32_t* lens = nullptr;
+  const void* q = nullptr;  // [rows, heads, dim]
+  int64_t q_row = 0, q_head = 0;
+  void* out = nullptr;
+  int64_t o_row = 0, o_head = 0;
+  float* lse = nullptr;  // [rows, heads] or null
+  int rows = 0, heads = 0, kv_heads = 0, dim = 0, page_size = 0, max_pages = 0, num_pages = 0;
+  float scale = 0.f;
+  int dtype = SLR_F32;
+  void* workspace = nullptr;
+  size_t workspace_bytes = 0;
+};
+int attend_workspace_size(int dtype, int dim, int rows, size_t* bytes);
+int launch_attend(const AttendArgs& a, cudaStream_t s);
+
+// New tokens' K and V into one layer's pages.
+struct AppendArgs {
+  void* k = nullptr;
+  void* v = nullptr;
+  int64_t page_stride = 0, head_stride = 0, token_stride = 0;
+  const int32_t* table = nullptr;
+  const int32_t* lens = nullptr;
+  const void* new_k = nullptr;  // [tokens, kv_heads, dim]
+  const void* new_v = nullptr;
+  int64_t k_row = 0, k_head = 0, v_row = 0, v_head = 0;
+  const int32_t* cu = nullptr;  // [rows + 1], or null: token i is row i's
+  int64_t tokens = 0;
+  int rows = 0, kv_heads = 0, dim = 0, page_size = 0, max_pages = 0, num_pages = 0;
+  int dtype = SLR_F32;
+};
+int launch_kv_append(const AppendArgs& a, cudaStream_t s);
+
+// Book-keeping of a cache and its pages as bytes: page p of plane i (a layer's
+// K or V) is page_bytes long at pool + planes[i] + p * page_stride.
+struct PagesArgs {
+  int32_t* state = nullptr;  // header, lens [rows], refs [pages], table [rows, max_pages]
+  int rows = 0, num_pages = 0, max_pages = 0, page_size = 0;
+  uint8_t* k = nullptr;  // layer 0
+  uint8_t* v = nullptr;
+  int64_t layer_bytes = 0, page_stride_bytes = 0, page_bytes = 0;
+  int layers = 0;
+  void* workspace = nullptr;
+};
+size_t kv_pages_workspace_size(int rows, int num_pages);
+int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const int32_t* parents, cudaStream_t s);
+int launch_kv_compact(const PagesArgs& p, cudaStream_t s);
+int launch_kv_copy(const PagesArgs& p, const int32_t* src, const int32_t* dst, int n, cudaStream_t s);
+
+// ---- log probabilities of tokens (k_logprobs.cu).
+struct LogprobArgs {
+  const void* logits = nullptr;
+  int64_t row_stride = 0, rows = 0, vocab = 0;
+  int dtype = SLR_F32;
+  const int64_t* targets = nullptr;
+  float* logprob = nullptr;
+  float* entropy = nullptr;
+  int top = 0;
+  int64_t* top_ids = nullptr;
+  float* top_logprobs = nullptr;
+};
+int launch_logprobs(const LogprobArgs& a, cudaStream_t s);
+int read_and_clear_status_attend(unsigned* out);
+int read_and_clear_status_pages(unsigned* out);
+int read_and_clear_status_logprobs(unsigned* out);
+
 // Device status words (bounded-wait timeouts) of each translation unit.
 int read_and_clear_status_mma(unsigned* out);
 int read_and_clear_status_tc(unsigned* out);

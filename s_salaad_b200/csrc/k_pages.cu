@@ -1,0 +1,584 @@
+// Book-keeping of a paged key-value cache on the device, so that a decode step
+// (also one replayed from a graph) never waits for the host: rows that fork,
+// end, roll back and grow; pages shared by reference and copied before they
+// are written; live pages moved to the lowest page numbers; new tokens'
+// keys and values written into their pages.
+//
+// All of it is bound by latency (a few thousand integers) except the page
+// copies, which are bound by HBM: 16-byte loads and stores, several in flight
+// per thread, over all layers' K and V at once.  Every choice is made in row
+// and page order, so the state never depends on timing; the only atomics are
+// integer sums and minima.
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "internal.hpp"
+
+namespace slr {
+
+__device__ unsigned g_status_pages;
+
+namespace {
+
+constexpr int kHeader = SLR_KV_HEADER_WORDS;
+enum : int { kShort = 0, kOver = 1, kCopies = 2, kLive = 3 };
+
+struct PagesK {
+  int32_t *head, *lens, *refs, *table;
+  int rows, num_pages, max_pages, page_size;
+  int32_t *growers, *first, *list, *src, *dst;  // workspace
+};
+
+__device__ __forceinline__ int64_t pages_of(int64_t len, int page_size) { return (len + page_size - 1) / page_size; }
+
+// Length of row r after the selection and before growth, clipped to the table.
+__device__ __forceinline__ int64_t kept_length(const PagesK& p, const int32_t* parents, const int32_t* n_new, int n_all,
+                                               int r, bool* bad) {
+  int from = parents ? parents[r] : r;
+  if (from >= p.rows) {
+    *bad = true;
+    from = -1;
+  }
+  if (from < 0) return 0;
+  int64_t len = p.lens[from];
+  const int64_t cap = int64_t(p.max_pages) * p.page_size;
+  if (len < 0 || len > cap) {
+    *bad = true;
+    len = len < 0 ? 0 : cap;
+  }
+  const int64_t n = n_new ? n_new[r] : n_all;
+  return n < 0 ? (len + n < 0 ? 0 : len + n) : len;
+}
+
+// Table rows become their parents' rows, entries behind the kept length -1.
+// Columns are independent, so a CTA reads its columns of every row before it
+// writes them: in place, one launch.  refs follow by integer atomics; each
+// CTA adds its change of the number of live pages.
+__global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32_t* parents, const int32_t* n_new,
+                                                     int n_all, int cols) {
+  extern __shared__ int32_t sm[];
+  int32_t* old = sm;                    // [rows][cols]
+  int32_t* keep = old + p.rows * cols;  // [rows] entries kept
+  int32_t* from = keep + p.rows;        // [rows]
+  __shared__ int s_most, s_live;
+  const int tid = threadIdx.x;
+  if (tid == 0) s_most = 0, s_live = 0;
+  __syncthreads();
+  bool bad = false;
+  int most = 0;
+  for (int r = tid; r < p.rows; r += blockDim.x) {
+    keep[r] = int(pages_of(kept_length(p, parents, n_new, n_all, r, &bad), p.page_size));
+    const int f = parents ? parents[r] : r;
+    from[r] = f >= p.rows ? -1 : f;
+    const int64_t len = p.lens[r];
+    most = max(most, int(min(int64_t(p.max_pages), pages_of(max(len, int64_t(0)), p.page_size))));
+  }
+  atomicMax(&s_most, most);
+  if (bad && blockIdx.x == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+  __syncthreads();
+  const int c0 = blockIdx.x * cols;
+  // no row has an entry from here on: there is nothing to move or to drop
+  if (c0 >= s_most) return;
+  for (int i = tid; i < p.rows * cols; i += blockDim.x) {
+    const int r = i / cols, c = c0 + i % cols;
+    old[i] = c < p.max_pages ? p.table[int64_t(r) * p.max_pages + c] : -1;
+  }
+  __syncthreads();
+  int live = 0;
+  for (int i = tid; i < p.rows * cols; i += blockDim.x) {
+    const int r = i / cols, j = i % cols, c = c0 + j;
+    if (c >= p.max_pages) continue;
+    const int was = old[i];
+    const int now = from[r] >= 0 && c < keep[r] ? old[from[r] * cols + j] : -1;
+    if (was == now) continue;
+    p.table[int64_t(r) * p.max_pages + c] = now;
+    if (was >= p.num_pages || now >= p.num_pages) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+    // a page is live while its count is above 0: the crossings add up to the net change
+    if (now >= 0 && now < p.num_pages) live += atomicAdd(p.refs + now, 1) == 0;
+    if (was >= 0 && was < p.num_pages) live -= atomicAdd(p.refs + was, -1) == 1;
+  }
+  if (live) atomicAdd(&s_live, live);
+  __syncthreads();
+  if (tid == 0 && s_live) atomicAdd(p.head + kLive, s_live);
+}
+
+constexpr int kGrowThreads = 1024;
+
+// Exclusive scan over the block; *total: the sum.  Ends with a barrier.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t* total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int64_t incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[w] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+  for (int i = 0; i < kGrowThreads / 32; ++i) {
+    const int64_t x = warp_sums[i];
+    before += i < w ? x : 0;
+    all += x;
+  }
+  *total = all;
+  return before + incl - v;
+}
+
+// Growth of every row: one CTA.  Pages are given out lowest number first in
+// row order, a row's copy of a shared last page before its new pages.
+__global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, const int32_t* parents,
+                                                            const int32_t* n_new, int n_all) {
+  extern __shared__ int32_t sm[];
+  int32_t* low = sm;              // [rows] kept lengths
+  int32_t* start = low + p.rows;  // [rows + 1] pages given to the rows before
+  int32_t* copy = start + p.rows + 1;
+  __shared__ int64_t warp_sums[kGrowThreads / 32];
+  __shared__ int s_over, s_bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) s_over = 0, s_bad = 0;
+  __syncthreads();
+  const int64_t cap = int64_t(p.max_pages) * p.page_size;
+  bool bad = false;
+  auto grow_of = [&](int r) -> int64_t {
+    const int64_t n = n_new ? n_new[r] : n_all;
+    return n <= 0 || (!n_new && low[r] == 0) ? 0 : n;  // one number for all: rows that hold tokens
+  };
+  for (int r = tid; r < p.rows; r += kGrowThreads) low[r] = int(kept_length(p, parents, n_new, n_all, r, &bad));
+  __syncthreads();
+  // rows about to write into a shared last page
+  auto shared_last = [&](int r) -> int {
+    if (grow_of(r) == 0 || low[r] % p.page_size == 0) return -1;
+    const int last = p.table[int64_t(r) * p.max_pages + low[r] / p.page_size];
+    if (last < 0 || last >= p.num_pages) {
+      bad = true;
+      return -1;
+    }
+    return p.refs[last] > 1 ? last : -1;
+  };
+  for (int r = tid; r < p.rows; r += kGrowThreads) {
+    const int last = shared_last(r);
+    copy[r] = last;
+    if (last >= 0) p.growers[last] = 0, p.first[last] = INT_MAX;
+    if (low[r] + grow_of(r) > cap) atomicAdd(&s_over, 1);
+  }
+  __syncthreads();
+  for (int r = tid; r < p.rows; r += kGrowThreads)
+    if (copy[r] >= 0) {
+      atomicAdd(p.growers + copy[r], 1);
+      atomicMin(p.first + copy[r], r);
+    }
+  __syncthreads();
+  // when every sharer grows, the lowest row keeps the page
+  const int chunk = (p.rows + kGrowThreads - 1) / kGrowThreads;
+  const int r0 = min(p.rows, tid * chunk), r1 = min(p.rows, r0 + chunk);
+  int64_t mine = 0;
+  auto need_of = [&](int r) -> int64_t {
+    return pages_of(low[r] + grow_of(r), p.page_size) - pages_of(low[r], p.page_size) + (copy[r] >= 0 ? 1 : 0);
+  };
+  for (int r = r0; r < r1; ++r) {
+    if (copy[r] >= 0 && __ldcg(p.growers + copy[r]) == __ldcg(p.refs + copy[r]) && __ldcg(p.first + copy[r]) == r)
+      copy[r] = -1;
+    mine += need_of(r);
+  }
+  int64_t total = 0;
+  int64_t at = block_scan(mine, warp_sums, &total);
+  const int over = s_over;
+  bool fits = over == 0 && total <= p.num_pages;
+  if (fits)
+    for (int r = r0; r < r1; ++r) {
+      start[r] = int(at);
+      at += need_of(r);
+    }
+  if (tid == 0) start[p.rows] = int(total);
+  // the lowest `total` free pages
+  int64_t found = 0;
+  if (total > 0) {
+    constexpr int kPer = 8;
+    for (int64_t base = 0; base < p.num_pages && (found < total || !fits); base += kGrowThreads * kPer) {
+      const int64_t i0 = base + tid * kPer;
+      unsigned mask = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (i0 + j < p.num_pages && __ldcg(p.refs + i0 + j) == 0) mask |= 1u << j;
+      int64_t sum = 0;
+      int64_t k = found + block_scan(__popc(mask), warp_sums, &sum);
+      if (fits)
+        for (int j = 0; j < kPer; ++j)
+          if (mask >> j & 1u) {
+            if (k < total) p.list[k] = int32_t(i0 + j);
+            ++k;
+          }
+      found += sum;
+    }
+  }
+  fits = fits && found >= total;
+  __syncthreads();
+  if (bad) s_bad = 1;
+  if (fits) {
+    for (int k = tid; k < total; k += kGrowThreads) {
+      int lo = 0, hi = p.rows - 1;  // the last row that starts at or before k and takes a page
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= k) lo = mid;
+        else hi = mid - 1;
+      }
+      const int r = lo, page = p.list[k];
+      int j = k - start[r] - (copy[r] >= 0 ? 1 : 0);
+      const int64_t col = pages_of(low[r], p.page_size) + j;  // j == -1: the copied page
+      p.table[int64_t(r) * p.max_pages + col] = page;
+      p.refs[page] = 1;
+    }
+    // the copies, in row order
+    int64_t copies = 0, n_mine = 0;
+    for (int r = r0; r < r1; ++r) n_mine += copy[r] >= 0;
+    int64_t c = block_scan(n_mine, warp_sums, &copies);
+    for (int r = r0; r < r1; ++r)
+      if (copy[r] >= 0) {
+        p.src[c] = copy[r];
+        p.dst[c] = p.list[start[r]];
+        ++c;
+        atomicAdd(p.refs + copy[r], -1);  // another row keeps it
+      }
+    for (int r = tid; r < p.rows; r += kGrowThreads) p.lens[r] = int(low[r] + grow_of(r));
+    if (tid == 0) {
+      p.head[kShort] = 0;
+      p.head[kOver] = 0;
+      p.head[kCopies] = int(copies);
+      p.head[kLive] += int(total);
+    }
+  } else {
+    for (int r = tid; r < p.rows; r += kGrowThreads) p.lens[r] = low[r];
+    if (tid == 0) {
+      p.head[kShort] = int(max(int64_t(0), min(int64_t(INT_MAX), total - found)));
+      p.head[kOver] = over;
+      p.head[kCopies] = 0;
+    }
+  }
+  __syncthreads();
+  if (tid == 0 && s_bad) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+}
+
+// Plan of a compaction: one CTA.  Live pages from the live count on go to the
+// free numbers below it, both ascending: no page is both read and written.
+__global__ void __launch_bounds__(kGrowThreads, 1) compact_plan_kernel(const PagesK p) {
+  __shared__ int64_t warp_sums[kGrowThreads / 32];
+  const int tid = threadIdx.x;
+  constexpr int kPer = 8;
+  int64_t mine = 0, live = 0;
+  for (int64_t i = tid; i < p.num_pages; i += kGrowThreads) mine += p.refs[i] > 0;
+  block_scan(mine, warp_sums, &live);
+  int64_t holes = 0, movers = 0;
+  for (int64_t base = 0; base < p.num_pages; base += kGrowThreads * kPer) {
+    const int64_t i0 = base + tid * kPer;
+    unsigned hole = 0, mover = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (i0 + j < p.num_pages) {
+        const bool used = p.refs[i0 + j] > 0;
+        if (i0 + j < live && !used) hole |= 1u << j;
+        if (i0 + j >= live && used) mover |= 1u << j;
+        if (i0 + j >= live) p.first[i0 + j] = -1;
+      }
+    // both counts in one scan
+    int64_t sum = 0;
+    const int64_t at = block_scan(int64_t(__popc(hole)) << 32 | __popc(mover), warp_sums, &sum);
+    int64_t h = holes + (at >> 32), m = movers + (at & 0xffffffff);
+    for (int j = 0; j < kPer; ++j) {
+      if (hole >> j & 1u) p.dst[h++] = int32_t(i0 + j);
+      if (mover >> j & 1u) p.src[m++] = int32_t(i0 + j);
+    }
+    holes += sum >> 32;
+    movers += sum & 0xffffffff;
+  }
+  __syncthreads();
+  for (int64_t i = tid; i < movers; i += kGrowThreads) {
+    const int s = p.src[i], d = p.dst[i];
+    p.refs[d] = p.refs[s];
+    p.refs[s] = 0;
+    p.first[s] = d;
+  }
+  if (tid == 0) {
+    p.head[kShort] = 0;
+    p.head[kOver] = 0;
+    p.head[kCopies] = int(movers);
+    p.head[kLive] = int(live);
+  }
+}
+
+struct CopyK {
+  uint8_t *k, *v;
+  int64_t layer_bytes, page_stride, page_bytes;
+  int planes, num_pages;
+  const int32_t *src, *dst;
+  const int32_t* count;  // device word, or null: n
+  int n;
+  bool check;            // pairs from the caller: those that could clash are left out
+  int32_t* table;        // compaction: entries to rewrite through `to`, or null
+  const int32_t* to;
+  const int32_t* live;
+  int64_t entries;
+};
+
+constexpr int kCopyThreads = 256;
+constexpr int kCopyUnroll = 4;
+
+template <int V> struct vec_of;
+template <> struct vec_of<16> { using type = uint4; };
+template <> struct vec_of<4> { using type = uint32_t; };
+
+// Pages src[i] -> dst[i] of every plane.  An item is a piece of one page of
+// one plane; CTAs take the items in turn.
+template <int V>
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyK a) {
+  using Vec = typename vec_of<V>::type;
+  pdl_wait_primary();
+  const int tid = threadIdx.x;
+  if (a.table) {
+    const int live = *a.live;
+    for (int64_t i = int64_t(blockIdx.x) * kCopyThreads + tid; i < a.entries; i += int64_t(gridDim.x) * kCopyThreads) {
+      const int e = a.table[i];
+      if (e < live) continue;
+      const int d = e < a.num_pages ? a.to[e] : -1;
+      if (d >= 0) a.table[i] = d;
+      else atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+    }
+  }
+  const int n = a.count ? *a.count : a.n;
+  constexpr int64_t kPiece = int64_t(kCopyThreads) * kCopyUnroll * V;
+  const int64_t pieces = (a.page_bytes + kPiece - 1) / kPiece;
+  const int64_t per_pair = pieces * a.planes;
+  int last = -1;
+  bool ok = true;
+  for (int64_t item = blockIdx.x; item < per_pair * n; item += gridDim.x) {
+    const int pair = int(item / per_pair);
+    const int64_t rest = item % per_pair;
+    const int plane = int(rest / pieces);
+    const int64_t off = (rest % pieces) * kPiece;
+    const int s = a.src[pair], d = a.dst[pair];
+    if (a.check && pair != last) {
+      last = pair;
+      bool clash = uint32_t(s) >= uint32_t(a.num_pages) || uint32_t(d) >= uint32_t(a.num_pages);
+      for (int i = tid; i < n; i += kCopyThreads) {
+        const int si = a.src[i], di = a.dst[i];
+        if (i != pair && si != di && s != d && (di == d || di == s || si == d)) clash = true;
+      }
+      ok = !__syncthreads_or(clash);
+      if (!ok && tid == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+    }
+    if (!ok || s == d) continue;
+    uint8_t* plane_base = ((plane & 1) ? a.v : a.k) + int64_t(plane >> 1) * a.layer_bytes;
+    const uint8_t* from = plane_base + int64_t(s) * a.page_stride + off;
+    uint8_t* to = plane_base + int64_t(d) * a.page_stride + off;
+    const int64_t left = a.page_bytes - off;
+    Vec x[kCopyUnroll];
+#pragma unroll
+    for (int i = 0; i < kCopyUnroll; ++i) {
+      const int64_t at = (int64_t(i) * kCopyThreads + tid) * V;
+      if (at < left) x[i] = *reinterpret_cast<const Vec*>(from + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kCopyUnroll; ++i) {
+      const int64_t at = (int64_t(i) * kCopyThreads + tid) * V;
+      if (at < left) *reinterpret_cast<Vec*>(to + at) = x[i];
+    }
+  }
+}
+
+// New tokens into their pages: one warp per token, 16-byte chunks (V = 16) or
+// single elements where the caller's rows are not aligned (V = element size).
+template <int V>
+__global__ void __launch_bounds__(128) append_kernel(const AppendArgs a, int esize) {
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t token = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (token >= a.tokens) return;
+  int row = int(token);
+  int64_t pos;
+  if (a.cu) {
+    // 32-ary search for the last row that starts at or before the token
+    int lo = 0, hi = a.rows;  // cu[lo] <= token < cu[hi] (cu[rows] = all tokens)
+    if (token >= a.cu[a.rows] || token < a.cu[0]) return;  // behind the last row
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32;
+      const int at = lo + lane * step;
+      const unsigned below = __ballot_sync(0xffffffffu, at < hi && a.cu[at] <= token);
+      const int k = below ? 31 - __clz(below) : 0;
+      const int nlo = lo + k * step;
+      hi = min(hi, nlo + step);
+      lo = nlo;
+    }
+    row = lo;
+    pos = int64_t(a.lens[row]) - (a.cu[row + 1] - token);
+    if (pos < 0) {
+      if (lane == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+      return;
+    }
+  } else {
+    pos = int64_t(a.lens[row]) - 1;
+    if (pos < 0) return;  // an empty row
+  }
+  if (pos >= int64_t(a.max_pages) * a.page_size) {
+    if (lane == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+    return;
+  }
+  const int page = a.table[int64_t(row) * a.max_pages + pos / a.page_size];
+  if (page < 0 || page >= a.num_pages) {
+    if (lane == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+    return;
+  }
+  const int64_t base = int64_t(page) * a.page_stride + (pos % a.page_size) * a.token_stride;
+  const int E = V / esize;
+  const int chunks = a.dim / E, all = a.kv_heads * chunks;
+  using Vec = std::conditional_t<V == 16, uint4, std::conditional_t<V == 4, uint32_t, unsigned short>>;
+  const uint8_t* nk = static_cast<const uint8_t*>(a.new_k);
+  const uint8_t* nv = static_cast<const uint8_t*>(a.new_v);
+  uint8_t* pk = static_cast<uint8_t*>(a.k);
+  uint8_t* pv = static_cast<uint8_t*>(a.v);
+#pragma unroll 4
+  for (int i = lane; i < all; i += 32) {
+    const int h = i / chunks, d = (i - h * chunks) * E;
+    const int64_t dst = (base + h * a.head_stride + d) * esize;
+    const Vec x = *reinterpret_cast<const Vec*>(nk + (token * a.k_row + h * a.k_head + d) * esize);
+    const Vec y = *reinterpret_cast<const Vec*>(nv + (token * a.v_row + h * a.v_head + d) * esize);
+    *reinterpret_cast<Vec*>(pk + dst) = x;
+    *reinterpret_cast<Vec*>(pv + dst) = y;
+  }
+}
+
+int sm_count(int* out) {
+  int dev = 0;
+  SLR_CHECK_CUDA(cudaGetDevice(&dev));
+  SLR_CHECK_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  return SLR_OK;
+}
+
+PagesK views(const PagesArgs& p) {
+  PagesK k = {};
+  k.head = p.state;
+  k.lens = k.head + kHeader;
+  k.refs = k.lens + p.rows;
+  k.table = k.refs + p.num_pages;
+  k.rows = p.rows;
+  k.num_pages = p.num_pages;
+  k.max_pages = p.max_pages;
+  k.page_size = p.page_size;
+  int32_t* w = static_cast<int32_t*>(p.workspace);
+  const int64_t pages = p.num_pages, pairs = std::max(p.rows, p.num_pages);
+  k.growers = w;
+  k.first = w + pages;
+  k.list = w + 2 * pages;
+  k.src = w + 3 * pages;
+  k.dst = w + 3 * pages + pairs;
+  return k;
+}
+
+int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, cudaStream_t s) {
+  c.k = p.k;
+  c.v = p.v;
+  c.layer_bytes = p.layer_bytes;
+  c.page_stride = p.page_stride_bytes;
+  c.page_bytes = p.page_bytes;
+  c.planes = 2 * p.layers;
+  c.num_pages = p.num_pages;
+  int sms = 0;
+  int rc = sm_count(&sms);
+  if (rc) return rc;
+  const int64_t pieces = ceil_div(p.page_bytes, int64_t(kCopyThreads) * kCopyUnroll * 16);
+  const int64_t items = std::max<int64_t>(1, pieces * c.planes * most_pairs);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(items, int64_t(sms) * 8)));
+  cfg.blockDim = dim3(kCopyThreads);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, copy_kernel<16>, c));
+  return SLR_OK;
+}
+
+}  // namespace
+
+size_t kv_pages_workspace_size(int rows, int num_pages) {
+  return size_t(4) * (3 * size_t(num_pages) + 2 * size_t(std::max(rows, num_pages)));
+}
+
+int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const int32_t* parents, cudaStream_t s) {
+  const PagesK k = views(p);
+  if (parents || n_new || n_all < 0) {
+    const int cols = p.rows <= 512 ? 32 : 8;
+    const size_t smem = (size_t(p.rows) * cols + 2 * size_t(p.rows)) * 4;
+    // one limit for every size, so that concurrent callers set the same
+    constexpr int kMost = std::max(512 * 34, kAttendMaxRows * 10) * 4;
+    SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    select_kernel<<<unsigned(ceil_div(p.max_pages, cols)), 256, smem, s>>>(k, parents, n_new, n_all, cols);
+    SLR_CHECK_LAUNCH("kv select");
+  }
+  const size_t smem = (3 * size_t(p.rows) + 1) * 4;
+  grow_kernel<<<1, kGrowThreads, smem, s>>>(k, parents, n_new, n_all);
+  SLR_CHECK_LAUNCH("kv grow");
+  CopyK c = {};
+  c.src = k.src;
+  c.dst = k.dst;
+  c.count = k.head + kCopies;
+  return copy_launch(p, c, p.rows, s);
+}
+
+int launch_kv_compact(const PagesArgs& p, cudaStream_t s) {
+  const PagesK k = views(p);
+  compact_plan_kernel<<<1, kGrowThreads, 0, s>>>(k);
+  SLR_CHECK_LAUNCH("kv compact");
+  CopyK c = {};
+  c.src = k.src;
+  c.dst = k.dst;
+  c.count = k.head + kCopies;
+  c.table = k.table;
+  c.to = k.first;
+  c.live = k.head + kLive;
+  c.entries = int64_t(p.rows) * p.max_pages;
+  return copy_launch(p, c, std::max<int64_t>(p.num_pages / 2, ceil_div(c.entries, 1024)), s);
+}
+
+int launch_kv_copy(const PagesArgs& p, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
+  CopyK c = {};
+  c.src = src;
+  c.dst = dst;
+  c.n = n;
+  c.check = true;
+  return copy_launch(p, c, n, s);
+}
+
+int launch_kv_append(const AppendArgs& a, cudaStream_t s) {
+  const int e = int(dtype_size(a.dtype));
+  const auto even = [&](int64_t stride) { return stride * e % 16 == 0; };
+  const bool wide = aligned16(a.new_k) && aligned16(a.new_v) && even(a.k_row) && even(a.k_head) && even(a.v_row) &&
+                    even(a.v_head) && a.dim * e % 16 == 0;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ceil_div(a.tokens, 4)));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (wide) SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel<16>, a, e));
+  else if (e == 4) SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel<4>, a, e));
+  else SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel<2>, a, e));
+  return SLR_OK;
+}
+
+int read_and_clear_status_pages(unsigned* out) {
+  unsigned v = 0, zero = 0;
+  SLR_CHECK_CUDA(cudaMemcpyFromSymbol(&v, g_status_pages, sizeof(v)));
+  if (v) SLR_CHECK_CUDA(cudaMemcpyToSymbol(g_status_pages, &zero, sizeof(zero)));
+  *out = v;
+  return SLR_OK;
+}
+
+}  // namespace slr

@@ -219,7 +219,12 @@ int slr_device_status(int* status_out) {
   rc = read_and_clear_status_dec(&w);
   if (rc) return rc;
   v |= w;
-  *status_out = (v & SLR_TIMEOUT_BIT) ? SLR_ERR_TIMEOUT : SLR_OK;
+  for (auto* read : {read_and_clear_status_attend, read_and_clear_status_pages, read_and_clear_status_logprobs}) {
+    rc = read(&w);
+    if (rc) return rc;
+    v |= w;
+  }
+  *status_out = (v & SLR_TIMEOUT_BIT) ? SLR_ERR_TIMEOUT : (v & SLR_BAD_INDEX_BIT) ? SLR_ERR_BAD_INDEX : SLR_OK;
   return SLR_OK;
 }
 

@@ -9,11 +9,15 @@
   that read one input, :class:`LayerSet` for independent layers side by side.
   Within :func:`single_launch_decode` (off by default), calls of 1 to 32
   tokens run the single-launch decode kernel (``slr_lrs_linear_decode``).
+* :func:`token_logprobs` — log probabilities of given tokens, entropy and the
+  best tokens of every row of logits.  (The paged key-value cache and its
+  attention are in :mod:`s_salaad_b200.kvcache`.)
 """
 from __future__ import annotations
 
 import contextlib
 import ctypes
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -652,6 +656,69 @@ def lrs_linear_forward(desc: LayerDesc, x: torch.Tensor) -> torch.Tensor:
     if not x2.is_contiguous():
         x2 = x2.contiguous()
     return desc.forward(x2).reshape(*shape[:-1], desc.out_features)
+
+
+# ------------------------------------------------------ scores of tokens --
+
+class TokenLogprobs(NamedTuple):
+    """Result of :func:`token_logprobs`; float32, except ``top_ids`` (int64).
+    What was not asked for is None."""
+
+    logprob: torch.Tensor | None       # [...] of the targets
+    entropy: torch.Tensor | None       # [...]
+    top_ids: torch.Tensor | None       # [..., top]
+    top_logprobs: torch.Tensor | None  # [..., top]
+
+
+def _no_graph(name: str, *tensors: torch.Tensor) -> None:
+    """The library's operators compute values only: refuse inputs that a
+    gradient would be expected of, instead of dropping it."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no backward pass; call it under torch.no_grad() or on detached tensors")
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top: int = 0,
+                   entropy: bool = True) -> TokenLogprobs:
+    """Scores under ``softmax(logits)``, logits ``[..., vocab]`` (CUDA, fp32 /
+    fp16 / bf16, unit stride in the last dimension), in one pass over them:
+    the log probability of ``targets`` (int64 ``[...]``; 0 where negative,
+    e.g. -100 for padding), the entropy, and the ``top`` (0..32) best tokens
+    with their log probabilities, greatest first, equal values by lower index.
+
+    Sums are float32.  -inf logits are tokens of probability 0; a row with a
+    NaN or +inf, or of -inf alone, gives NaN (as ``torch.log_softmax``).  A
+    target from vocab on gives NaN and ``SLR_ERR_BAD_INDEX`` from
+    ``slr_device_status`` (the call itself does not wait for the GPU).
+    """
+    lib = _lib.load()
+    _require_cuda("logits", logits)
+    dtype = slr_dtype(logits.dtype)
+    if logits.dim() < 1:
+        raise ValueError("logits must have at least one dimension")
+    vocab = logits.shape[-1]
+    if not 0 <= top <= min(_lib.SLR_MAX_TOP, vocab):
+        raise ValueError(f"top must be in [0, min({_lib.SLR_MAX_TOP}, vocab)], got {top}")
+    if targets is not None:
+        if targets.dtype != torch.int64:
+            raise TypeError(f"targets must be int64, got {targets.dtype}")
+        if targets.device != logits.device or targets.shape != logits.shape[:-1]:
+            raise ValueError(f"targets must be {tuple(logits.shape[:-1])} on {logits.device}")
+        targets = targets.contiguous()
+    _no_graph("token_logprobs", logits)
+    shape, dev = logits.shape[:-1], logits.device
+    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < vocab):
+        x = x.contiguous()
+    rows = x.shape[0]
+    lp = torch.empty(shape, dtype=torch.float32, device=dev) if targets is not None else None
+    ent = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
+    ids = torch.empty(*shape, top, dtype=torch.int64, device=dev) if top else None
+    val = torch.empty(*shape, top, dtype=torch.float32, device=dev) if top else None
+    with _DeviceGuard(dev):
+        rc = lib.slr_token_logprobs(x.data_ptr(), x.stride(0) if rows > 1 else vocab, rows, vocab, dtype,
+                                    _ptr(targets), _ptr(lp), _ptr(ent), top, _ptr(ids), _ptr(val), _stream(dev))
+    _lib.check(rc, "token_logprobs")
+    return TokenLogprobs(lp, ent, ids, val)
 
 
 # ---------------------------------------------------------- dense -> BSR --
