@@ -222,7 +222,7 @@ _SIGS = {
     "slr_nm_linear_workspace_size": ([ctypes.POINTER(SlrNmLayer), i64], sz),
     "slr_nm_linear_forward": ([ctypes.POINTER(SlrNmLayer), vp, i64, vp, i64, i64, vp, sz, vp], i32),
     "slr_kv_pages_workspace_size": ([ctypes.POINTER(SlrKvCache)], sz),
-    "slr_kv_attend_workspace_size": ([ctypes.POINTER(SlrKvCache)], sz),
+    "slr_kv_attend_workspace_size": ([ctypes.POINTER(SlrKvCache), ctypes.c_int32, ctypes.c_int32], sz),
     "slr_kv_advance": ([ctypes.POINTER(SlrKvCache), vp, vp, ctypes.c_int32, vp, sz, vp], i32),
     "slr_kv_compact": ([ctypes.POINTER(SlrKvCache), vp, sz, vp], i32),
     "slr_kv_copy_pages": ([ctypes.POINTER(SlrKvCache), vp, vp, ctypes.c_int32, vp], i32),

@@ -49,7 +49,7 @@ struct AttendK {
   float* part_o;     // [2 * ctas][GT][DP]
   float2* part_ml;   // [2 * ctas][GT]
   int32_t* prefix;   // [rows + 1] tiles before each row
-  int rows, kv_heads, group, hblocks, dim, page_size, max_pages, num_pages, ctas;
+  int rows, kv_heads, group, hblocks, dim, page_size, page_shift, max_pages, num_pages, ctas;
   float scale_log2;
 };
 
@@ -60,14 +60,25 @@ __device__ __forceinline__ int64_t tiles_per_cta(int64_t n, int ctas, int min_ti
   return per < min_tiles ? min_tiles : per;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool fill) {
-  // src-size 0 writes 16 zero bytes and reads nothing
-  const int n = fill ? 16 : 0;
+// 16 bytes, or (n = 0) 16 zero bytes without reading.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int n) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Transposes an 8 x 8 matrix of 16-bit elements held one row per four lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 
 template <typename T> struct pair_of;
@@ -86,29 +97,30 @@ template <> struct pair_of<__half> {
   __device__ static float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 };
 
-// Shape of one instance: DP head dimension padded to a power of two, W warps,
-// TT tokens per warp and tile, NS stages per warp, GT query heads per CTA, RB
-// rows of them joined per round.
-template <typename T, int DP_> struct Cfg {
+// Shape of one instance: DP head dimension padded to a power of two, GT query
+// heads per CTA, W warps, TT tokens per warp and tile, NS stages per warp.
+// Two CTAs of 96 KB at DP = 128: 128 KB of loads in flight per SM.
+template <typename T, int DP_, int GT_> struct Cfg {
   static constexpr bool kF32 = std::is_same<T, float>::value;
-  static constexpr int DP = DP_;
+  static constexpr int DP = DP_, GT = GT_;
   static constexpr int W = 4;
   static constexpr int TT = kF32 ? 8 : 16;
   static constexpr int NS = DP == 64 ? 4 : 3;
-  static constexpr int GT = kF32 ? 8 : 16;
-  static constexpr int RB = kF32 ? 4 : 8;
+  static constexpr int RB = GT < 8 ? GT : 8;           // heads joined per round at the end of a row
   static constexpr int kTile = W * TT;
   static constexpr int kRow = DP * int(sizeof(T));     // bytes of a token's row
   static constexpr int kHalf = TT * kRow;              // K (or V) bytes of a stage
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kRing = W * NS * kStage;
-  static constexpr int kBuf = (W - 1) * RB * DP * 4;   // other warps' o at the end of a row
+  static constexpr int kObuf = DP + 4;                 // floats of a head's row in the join (bank offset 4)
   static constexpr int kMl = W * GT * 8;
-  static constexpr int kQ = kF32 ? GT * DP * 4 : 0;
+  static constexpr bool kQRegs = GT * DP <= 256;       // fp32: a lane's quarter of q in registers
+  static constexpr int kQ = kF32 && !kQRegs ? GT * DP * 4 : 0;
   static constexpr int kP = kF32 ? W * TT * GT * 4 : 0;
   static constexpr int kCnt = W * NS * 4;
-  static constexpr int kFixed = kRing + kBuf + kMl + kQ + kP + kCnt + 64;
+  static constexpr int kFixed = kRing + kMl + kQ + kP + kCnt + 64;
   static constexpr int kMinTiles = kF32 ? 4 : 2;
+  static_assert(RB * kObuf * 4 <= kStage, "the join's rows take a stage's place");
 };
 
 // Place in the list of tiles: row b, head block h, tile of the row.
@@ -129,18 +141,17 @@ __device__ __forceinline__ void cursor_next(Cursor& c, const int* lens, int rows
   c.ntiles = (c.len + kTile - 1) / kTile;
 }
 
-template <typename T, int DP_>
-__global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const AttendK a) {
-  using C = Cfg<T, DP_>;
+template <typename T, int DP_, int GT_>
+__global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const AttendK a) {
+  using C = Cfg<T, DP_, GT_>;
   constexpr int DP = C::DP, W = C::W, TT = C::TT, NS = C::NS, GT = C::GT, RB = C::RB;
   constexpr int kThreads = W * 32;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem;
-  float* buf = reinterpret_cast<float*>(smem + C::kRing);
-  float2* ml = reinterpret_cast<float2*>(smem + C::kRing + C::kBuf);
-  float* qs = reinterpret_cast<float*>(smem + C::kRing + C::kBuf + C::kMl);
-  float* ps = reinterpret_cast<float*>(smem + C::kRing + C::kBuf + C::kMl + C::kQ);
-  int* cnt = reinterpret_cast<int*>(smem + C::kRing + C::kBuf + C::kMl + C::kQ + C::kP);
+  float2* ml = reinterpret_cast<float2*>(smem + C::kRing);
+  float* qs = reinterpret_cast<float*>(smem + C::kRing + C::kMl);
+  float* ps = reinterpret_cast<float*>(smem + C::kRing + C::kMl + C::kQ);
+  int* cnt = reinterpret_cast<int*>(smem + C::kRing + C::kMl + C::kQ + C::kP);
   int* scratch = cnt + W * NS;                       // 16 words
   int* lens = reinterpret_cast<int*>(smem + C::kFixed);  // [rows]
 
@@ -211,13 +222,24 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
   int64_t seg_start = t_begin - c.tile;
 
   // ---- the ring
+  // Chunk `ch` of a token's row lies at ch ^ (row & 7): the eight rows of an
+  // ldmatrix (or the lanes of a 16-byte read) meet all banks once.
   const uint32_t ring_w = smem_u32(ring) + w * NS * C::kStage;
   int* cnt_w = cnt + w * NS;
+  auto kv_head = [&](int h) { return a.hblocks == 1 ? h : h / a.hblocks; };
+  auto page_of = [&](int t) { return a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size; };
   Cursor f = c;
   auto fetch_page = [&](const Cursor& u) -> int {
     const int t0 = u.tile * C::kTile + w * TT;
-    return t0 < u.len ? a.table[int64_t(u.b) * a.max_pages + t0 / a.page_size] : 0;
+    return t0 < u.len ? a.table[int64_t(u.b) * a.max_pages + page_of(t0)] : 0;
   };
+  constexpr int E = 16 / int(sizeof(T));             // elements of a 16-byte chunk
+  constexpr int CH = DP / E;                         // chunks of a row
+  constexpr int kRowStep = CH <= 32 ? 32 / CH : 1;   // rows that a warp-wide load covers
+  constexpr int kColStep = CH <= 32 ? 1 : CH / 32;   // warp-wide loads of one row
+  const int lrow = lane / CH, lch = lane % CH;
+  const uint32_t ldst = lrow * C::kRow + ((lch ^ lrow) << 4);
+  const int64_t lsrc = lrow * a.token_stride + lch * E;
   int page = fetch_page(f);
   int loaded = 0, load_slot = 0;
   auto load_stage = [&]() {
@@ -230,22 +252,38 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
       }
       if (lane == 0) cnt_w[load_slot] = valid;
       if (valid > 0) {
-        const int64_t off = int64_t(page) * a.page_stride + int64_t(f.h / a.hblocks) * a.head_stride +
-                            int64_t(t0 % a.page_size) * a.token_stride;
+        const int64_t off = int64_t(page) * a.page_stride + int64_t(kv_head(f.h)) * a.head_stride +
+                            int64_t(t0 - page_of(t0) * a.page_size) * a.token_stride + lsrc;
         const T* ks = static_cast<const T*>(a.k) + off;
         const T* vs = static_cast<const T*>(a.v) + off;
-        constexpr int E = 16 / int(sizeof(T));   // elements of a 16-byte chunk
-        constexpr int CH = DP / E;               // chunks of a row
-        const uint32_t base = ring_w + load_slot * C::kStage;
+        const uint32_t dst = ring_w + load_slot * C::kStage + ldst;
+        if (valid == TT && a.dim == DP) {
 #pragma unroll
-        for (int i = 0; i < TT * CH / 32; ++i) {
-          const int idx = i * 32 + lane;
-          const int row = idx / CH, ch = idx % CH;
-          const bool in = row < valid && ch * E < a.dim;
-          const uint32_t dst = base + row * C::kRow + ((ch ^ (row & 7)) << 4);
-          const int64_t src = in ? row * a.token_stride + ch * E : 0;
-          cp_async16(dst, ks + src, in);
-          cp_async16(dst + C::kHalf, vs + src, in);
+          for (int i = 0; i < TT / kRowStep; ++i) {
+#pragma unroll
+            for (int j = 0; j < kColStep; ++j) {
+              const uint32_t d = (dst + i * kRowStep * C::kRow + j * 512) ^ (((i * kRowStep) & 7) << 4);
+              cp_async16(d, ks + j * 32 * E, 16);
+              cp_async16(d + C::kHalf, vs + j * 32 * E, 16);
+            }
+            ks += kRowStep * a.token_stride;
+            vs += kRowStep * a.token_stride;
+          }
+        } else {
+          const T* k0 = static_cast<const T*>(a.k);
+          const T* v0 = static_cast<const T*>(a.v);
+#pragma unroll
+          for (int i = 0; i < TT / kRowStep; ++i) {
+#pragma unroll
+            for (int j = 0; j < kColStep; ++j) {
+              const bool in = lrow + i * kRowStep < valid && (lch + j * 32) * E < a.dim;
+              const uint32_t d = (dst + i * kRowStep * C::kRow + j * 512) ^ (((i * kRowStep) & 7) << 4);
+              cp_async16(d, in ? ks + j * 32 * E : k0, in ? 16 : 0);
+              cp_async16(d + C::kHalf, in ? vs + j * 32 * E : v0, in ? 16 : 0);
+            }
+            ks += kRowStep * a.token_stride;
+            vs += kRowStep * a.token_stride;
+          }
         }
       }
       ++loaded;
@@ -261,33 +299,46 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
   for (int i = 0; i < NS - 1; ++i) load_stage();
 
   // ---- running softmax of this warp: log2-domain maximum, sum, output
-  // 16-bit: rows lane/4 and lane/4 + 8 (index 0, 1), columns of the MMA tiles.
+  // 16-bit: the MMAs compute Sᵀ = K · Qᵀ (16 tokens x 8 heads) and Oᵀ = Vᵀ · Pᵀ
+  // (16 columns x 8 heads), so a lane has heads 2 (lane % 4) and + 1 of every
+  // 8 in both; groups of up to 8 heads waste no MMA on empty rows.
   // fp32: every lane all GT heads, DP / 32 columns each.
-  constexpr int kRows = C::kF32 ? GT : 2;
-  constexpr int kOut = C::kF32 ? GT * (DP / 32) : DP / 2;
-  float m[kRows], l[kRows], o[kOut];
-  uint32_t qf[C::kF32 ? 1 : DP / 4];
+  constexpr int NT = C::kF32 ? 1 : GT / 8;
+  constexpr int kStat = C::kF32 ? GT : 2 * NT;
+  constexpr int kOut = C::kF32 ? GT * (DP / 32) : NT * DP / 4;
+  float m[kStat], l[kStat], o[kOut];
+  uint32_t qf[C::kF32 ? 1 : NT * DP / 8];
+  float qr[C::kF32 && C::kQRegs ? GT * DP / 4 : 1];
   auto reset = [&]() {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) m[i] = -INFINITY, l[i] = 0.f;
+    for (int i = 0; i < kStat; ++i) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < kOut; ++i) o[i] = 0.f;
   };
   auto load_q = [&]() {
-    const int kvh = c.h / a.hblocks, g0 = (c.h % a.hblocks) * GT;
+    const int kvh = kv_head(c.h), g0 = (c.h - kvh * a.hblocks) * GT;
     const T* q = static_cast<const T*>(a.q) + int64_t(c.b) * a.q_row + int64_t(kvh * a.group + g0) * a.q_head;
     const int heads = min(GT, a.group - g0);
     if constexpr (C::kF32) {
-      for (int i = tid; i < GT * DP; i += kThreads) {
-        const int g = i / DP, d = i % DP;
-        qs[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
+      if constexpr (C::kQRegs) {
+#pragma unroll
+        for (int i = 0; i < GT * DP / 4; ++i) {
+          const int g = i / (DP / 4), d = (lane >> 3) * (DP / 4) + i % (DP / 4);
+          qr[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
+        }
+      } else {
+        for (int i = tid; i < GT * DP; i += kThreads) {
+          const int g = i / DP, d = i % DP;
+          qs[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
+        }
+        __syncthreads();
       }
-      __syncthreads();
     } else {
       const unsigned short* qu = reinterpret_cast<const unsigned short*>(q);
 #pragma unroll
-      for (int i = 0; i < DP / 4; ++i) {
-        const int g = (lane >> 2) + (i & 1) * 8, d = (i >> 2) * 16 + (i & 2) * 4 + (lane & 3) * 2;
+      for (int i = 0; i < NT * DP / 8; ++i) {
+        // i = (k-step, head tile, half of the k-step)
+        const int g = (i >> 1) % NT * 8 + (lane >> 2), d = (i / (2 * NT)) * 16 + (i & 1) * 8 + (lane & 3) * 2;
         uint32_t v = 0;
         if (g < heads && d < a.dim) {
           const unsigned short* p = qu + g * a.q_head + d;
@@ -298,131 +349,140 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
     }
   };
 
-  auto step = [&](uint32_t base, int valid, bool two) {
+  auto step = [&](uint32_t base, int valid) {
     if constexpr (!C::kF32) {
-      float s[2][4] = {};
+      const int r8 = lane & 7;
+      float s[NT][2][4] = {};
+      {
+        const uint32_t at = base + (((lane >> 3) & 1) * 8 + r8) * C::kRow + (((lane >> 4) ^ r8) << 4);
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        const int row = ((lane >> 4) << 3) + (lane & 7), ch = ks * 2 + ((lane >> 3) & 1);
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4(base + row * C::kRow + ((ch ^ (row & 7)) << 4), b0, b1, b2, b3);
-        mma16816<T>::run(s[0], qf + ks * 4, b0, b1);
-        mma16816<T>::run(s[1], qf + ks * 4, b2, b3);
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          uint32_t k[4];
+          ldsm_x4(at ^ (ks << 5), k[0], k[1], k[2], k[3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)  // two chains: half the latency
+            mma16816<T>::run(s[nt][ks & 1], k, qf[(ks * NT + nt) * 2], qf[(ks * NT + nt) * 2 + 1]);
+        }
       }
-      // With scale < 0 the largest product is the smallest score: the maximum is taken after scaling.
-      float mn[2], f[2];
+      float mn[kStat];
+      bool grew = false;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float x = -INFINITY;
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int e = 0; e < 4; ++e) s[nt][0][e] += s[nt][1][e];
+        // With scale < 0 the largest product is the smallest score: the maximum is taken after scaling.
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int t = j * 8 + (lane & 3) * 2 + e;
-            x = fmaxf(x, t < valid ? s[j][r * 2 + e] * a.scale_log2 : -INFINITY);
+        for (int e = 0; e < 2; ++e) {
+          float x0 = s[nt][0][e] * a.scale_log2, x1 = s[nt][0][e + 2] * a.scale_log2;
+          if (valid < TT) {
+            if ((lane >> 2) >= valid) x0 = -INFINITY;
+            if ((lane >> 2) + 8 >= valid) x1 = -INFINITY;
           }
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        mn[r] = fmaxf(m[r], x);
+          float x = fmaxf(x0, x1);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          mn[nt * 2 + e] = fmaxf(m[nt * 2 + e], x);
+          grew |= mn[nt * 2 + e] > m[nt * 2 + e];
+        }
       }
-      const bool grew = mn[0] > m[0] || mn[1] > m[1];
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          f[r] = mn[r] == -INFINITY ? 1.f : exp2f(m[r] - mn[r]);
-          l[r] *= f[r];
-          m[r] = mn[r];
-        }
+        for (int nt = 0; nt < NT; ++nt) {
+          float fac[2];
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-          o[i * 4 + 0] *= f[0];
-          o[i * 4 + 1] *= f[0];
-          o[i * 4 + 2] *= f[1];
-          o[i * 4 + 3] *= f[1];
+          for (int e = 0; e < 2; ++e) {
+            const int i = nt * 2 + e;
+            fac[e] = mn[i] == m[i] ? 1.f : ex2(m[i] - mn[i]);
+            l[i] *= fac[e];
+            m[i] = mn[i];
+          }
+#pragma unroll
+          for (int i = 0; i < DP / 4; ++i) o[nt * (DP / 4) + i] *= fac[i & 1];
         }
       }
       // P as the sum of two 16-bit numbers (hi + lo): one alone would add an
       // error of the size of the output's own rounding.
-      uint32_t hi[4], lo[4];
+      uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float base_m = m[r] == -INFINITY ? 0.f : m[r];
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float top = m[nt * 2 + (e & 1)];
+          p[e] = ex2(fmaf(s[nt][0][e], a.scale_log2, top == -INFINITY ? 0.f : -top));
+          if (valid < TT && (lane >> 2) + (e >> 1) * 8 >= valid) p[e] = 0.f;
+          l[nt * 2 + (e & 1)] += p[e];
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float p0 = 0.f, p1 = 0.f;
-          if (r == 0 || two) {
-            const int t = j * 8 + (lane & 3) * 2;
-            if (t < valid) p0 = exp2f(fmaf(s[j][r * 2], a.scale_log2, -base_m));
-            if (t + 1 < valid) p1 = exp2f(fmaf(s[j][r * 2 + 1], a.scale_log2, -base_m));
-          }
-          l[r] += p0 + p1;
-          const uint32_t h = pair_of<T>::pack(p0, p1);
+          const uint32_t h = pair_of<T>::pack(p[j * 2], p[j * 2 + 1]);
           const float2 back = pair_of<T>::unpack(h);
-          hi[j * 2 + r] = h;
-          lo[j * 2 + r] = pair_of<T>::pack(p0 - back.x, p1 - back.y);
+          hi[nt][j] = transpose8(h);
+          lo[nt][j] = transpose8(pair_of<T>::pack(p[j * 2] - back.x, p[j * 2 + 1] - back.y));
         }
       }
+      const uint32_t at = base + C::kHalf + ((lane >> 4) * 8 + r8) * C::kRow + ((((lane >> 3) & 1) ^ r8) << 4);
 #pragma unroll
-      for (int nt = 0; nt < DP / 16; ++nt) {
-        const int row = (((lane >> 3) & 1) << 3) + (lane & 7), ch = nt * 2 + (lane >> 4);
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4_trans(base + C::kHalf + row * C::kRow + ((ch ^ (row & 7)) << 4), b0, b1, b2, b3);
-        mma16816<T>::run(o + nt * 8, hi, b0, b1);
-        mma16816<T>::run(o + nt * 8 + 4, hi, b2, b3);
-        mma16816<T>::run(o + nt * 8, lo, b0, b1);
-        mma16816<T>::run(o + nt * 8 + 4, lo, b2, b3);
+      for (int dt = 0; dt < DP / 16; ++dt) {
+        uint32_t v[4];
+        ldsm_x4_trans(at ^ (dt << 5), v[0], v[1], v[2], v[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<T>::run(o + nt * (DP / 4) + dt * 4, v, hi[nt][0], hi[nt][1]);
+          mma16816<T>::run(o + nt * (DP / 4) + dt * 4, v, lo[nt][0], lo[nt][1]);
+        }
       }
     } else {
       // lane = token (lane & 7) x quarter of the head dimension (lane >> 3)
       const int t = lane & 7, qt = lane >> 3;
-      const int heads = min(GT, a.group - (c.h % a.hblocks) * GT);
       float s[GT] = {};
-      const uint8_t* kr = ring + (base - smem_u32(ring)) + t * C::kRow;
+      const uint8_t* stage = ring + (base - smem_u32(ring));
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         const int ch = qt * (DP / 16) + i;
-        const float4 kv = *reinterpret_cast<const float4*>(kr + ((ch ^ t) << 4));
+        const float4 kv = *reinterpret_cast<const float4*>(stage + t * C::kRow + ((ch ^ t) << 4));
 #pragma unroll
-        for (int g = 0; g < GT; ++g)
-          if (g < heads) {
-            const float4 qv = *reinterpret_cast<const float4*>(qs + g * DP + ch * 4);
-            s[g] = fmaf(qv.x, kv.x, s[g]);
-            s[g] = fmaf(qv.y, kv.y, s[g]);
-            s[g] = fmaf(qv.z, kv.z, s[g]);
-            s[g] = fmaf(qv.w, kv.w, s[g]);
+        for (int g = 0; g < GT; ++g) {
+          float4 qv;
+          if constexpr (C::kQRegs) {
+            const float* x = qr + g * (DP / 4) + i * 4;
+            qv = make_float4(x[0], x[1], x[2], x[3]);
+          } else {
+            qv = *reinterpret_cast<const float4*>(qs + g * DP + ch * 4);
           }
+          s[g] = fmaf(qv.x, kv.x, s[g]);
+          s[g] = fmaf(qv.y, kv.y, s[g]);
+          s[g] = fmaf(qv.z, kv.z, s[g]);
+          s[g] = fmaf(qv.w, kv.w, s[g]);
+        }
       }
       float* pw = ps + w * TT * GT;
 #pragma unroll
-      for (int g = 0; g < GT; ++g)
-        if (g < heads) {
-          s[g] += __shfl_xor_sync(0xffffffffu, s[g], 8);
-          s[g] += __shfl_xor_sync(0xffffffffu, s[g], 16);
-          float x = t < valid ? s[g] * a.scale_log2 : -INFINITY;
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          const float mn = fmaxf(m[g], x);
-          if (mn > m[g]) {
-            const float fac = exp2f(m[g] - mn);
-            l[g] *= fac;
+      for (int g = 0; g < GT; ++g) {
+        s[g] += __shfl_xor_sync(0xffffffffu, s[g], 8);
+        s[g] += __shfl_xor_sync(0xffffffffu, s[g], 16);
+        float x = t < valid ? s[g] * a.scale_log2 : -INFINITY;
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        if (x > m[g]) {  // the same for all lanes
+          const float fac = ex2(m[g] - x);
+          l[g] *= fac;
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) o[g * (DP / 32) + i] *= fac;
-            m[g] = mn;
-          }
-          const float base_m = m[g] == -INFINITY ? 0.f : m[g];
-          const float p = t < valid ? exp2f(fmaf(s[g], a.scale_log2, -base_m)) : 0.f;
-          if (qt == 0) {
-            l[g] += p;
-            pw[t * GT + g] = p;
-          }
+          for (int i = 0; i < DP / 32; ++i) o[g * (DP / 32) + i] *= fac;
+          m[g] = x;
         }
+        const float p = t < valid ? ex2(fmaf(s[g], a.scale_log2, m[g] == -INFINITY ? 0.f : -m[g])) : 0.f;
+        if (qt == 0) {
+          l[g] += p;
+          pw[t * GT + g] = p;
+        }
+      }
       __syncwarp();
-      const uint8_t* vr = ring + (base - smem_u32(ring)) + C::kHalf;
-#pragma unroll
-      for (int tt = 0; tt < TT; ++tt) {
-        if (tt >= valid) break;
-        float vv[DP / 32];
+      const uint8_t* vr = stage + C::kHalf;
+      auto add = [&](int tt) {
+        float vv[DP / 32], pg[GT];
         if constexpr (DP == 64) {
           const float2 x = *reinterpret_cast<const float2*>(vr + tt * C::kRow + (((lane >> 1) ^ tt) << 4) + (lane & 1) * 8);
           vv[0] = x.x, vv[1] = x.y;
@@ -433,121 +493,94 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
             vv[j * 4] = x.x, vv[j * 4 + 1] = x.y, vv[j * 4 + 2] = x.z, vv[j * 4 + 3] = x.w;
           }
         }
-        const float4 pa = *reinterpret_cast<const float4*>(pw + tt * GT);
-        const float4 pb = *reinterpret_cast<const float4*>(pw + tt * GT + 4);
-        const float pg[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+        if constexpr (GT % 4 == 0) {
+#pragma unroll
+          for (int g = 0; g < GT; g += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(pw + tt * GT + g);
+            pg[g] = x.x, pg[g + 1] = x.y, pg[g + 2] = x.z, pg[g + 3] = x.w;
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < GT; ++g) pg[g] = pw[tt * GT + g];
+        }
 #pragma unroll
         for (int g = 0; g < GT; ++g)
-          if (g < heads)
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) o[g * (DP / 32) + i] = fmaf(pg[g], vv[i], o[g * (DP / 32) + i]);
-      }
+          for (int i = 0; i < DP / 32; ++i) o[g * (DP / 32) + i] = fmaf(pg[g], vv[i], o[g * (DP / 32) + i]);
+      };
+      // rows behind the length are zeros in the stage, their p is 0
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) add(tt);
       __syncwarp();
     }
   };
 
-  // One value pair of (row g, columns d, d + 1) or one column group of the
-  // joined output to its place.
-  auto finish = [&](int64_t seg0, int64_t seg1) {
+  // End of a row (or of this CTA's part): the warps' results are joined and
+  // written, final ones as output, parts of a split row to the workspace.
+  // The warps' rows lie in the place of the stage that each has just used.
+  auto finish = [&](int64_t seg0, int64_t seg1, int used) {
     const bool whole = seg0 >= t_begin && seg1 <= t_end;
-    const int slot = 2 * int(blockIdx.x) + (seg0 >= t_begin ? 1 : 0);
-    const int kvh = c.h / a.hblocks, g0 = (c.h % a.hblocks) * GT;
+    const int part = 2 * int(blockIdx.x) + (seg0 >= t_begin ? 1 : 0);
+    const int kvh = kv_head(c.h), g0 = (c.h - kvh * a.hblocks) * GT;
     const int heads = min(GT, a.group - g0);
-    // the sum of a row over the lanes that share it
+    // the sum of a head over the lanes that share it
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if constexpr (C::kF32) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 4);
-        l[r] = __shfl_sync(0xffffffffu, l[r], 0);
-      }
-    }
-    __syncthreads();  // warp 0 has read the previous row's buffers
+    for (int i = 0; i < kStat; ++i)
+#pragma unroll
+      for (int x = C::kF32 ? 1 : 4; x < (C::kF32 ? 8 : 32); x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
     if constexpr (C::kF32) {
       if (lane == 0)
 #pragma unroll
         for (int g = 0; g < GT; ++g) ml[w * GT + g] = make_float2(m[g], l[g]);
-    } else if ((lane & 3) == 0) {
-      ml[w * GT + (lane >> 2)] = make_float2(m[0], l[0]);
-      ml[w * GT + (lane >> 2) + 8] = make_float2(m[1], l[1]);
+    } else if (lane < 4) {
+#pragma unroll
+      for (int i = 0; i < kStat; ++i) ml[w * GT + (i >> 1) * 8 + lane * 2 + (i & 1)] = make_float2(m[i], l[i]);
     }
+    float* mine = reinterpret_cast<float*>(ring + (w * NS + used) * C::kStage);
 #pragma unroll
     for (int rb = 0; rb < GT / RB; ++rb) {
       if (rb * RB >= heads) break;
-      if (rb) __syncthreads();
-      if (w) {
-        float* dst = buf + (w - 1) * RB * DP;
-        if constexpr (C::kF32) {
+      if constexpr (C::kF32) {
 #pragma unroll
-          for (int r = 0; r < RB; ++r)
+        for (int r = 0; r < RB; ++r)
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-              const int d = DP == 64 ? lane * 2 + i : (i / 4) * 128 + lane * 4 + (i & 3);
-              dst[r * DP + d] = o[(rb * RB + r) * (DP / 32) + i];
-            }
+          for (int i = 0; i < DP / 32; ++i)
+            mine[r * C::kObuf + (DP == 64 ? lane * 2 + i : (i / 4) * 128 + lane * 4 + (i & 3))] =
+                o[(rb * RB + r) * (DP / 32) + i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < DP / 4; ++i)
+          mine[((lane & 3) * 2 + (i & 1)) * C::kObuf + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (lane >> 2)] =
+              o[rb * (DP / 4) + i];
+      }
+      __syncthreads();
+      for (int i = tid; i < RB * DP; i += kThreads) {
+        const int lr = i / DP, d = i % DP, g = rb * RB + lr;
+        if (g >= heads) break;
+        float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) top = fmaxf(top, ml[j * GT + g].x);
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const float2 x = ml[j * GT + g];
+          // a warp without a finite score has sum 0, or NaN if a score was NaN
+          const float fac = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : ex2(x.x - top);
+          sum = fmaf(x.y, fac, sum);
+          y = fmaf(reinterpret_cast<const float*>(ring + (j * NS + used) * C::kStage)[lr * C::kObuf + d], fac, y);
+        }
+        if (whole) {
+          const int head = kvh * a.group + g0 + g;
+          if (d < a.dim)
+            static_cast<T*>(a.out)[int64_t(c.b) * a.o_row + int64_t(head) * a.o_head + d] =
+                from_f<T>(sum == 0.f ? 0.f : y / sum);
+          if (d == 0 && a.lse)
+            a.lse[int64_t(c.b) * a.kv_heads * a.group + head] = sum == 0.f ? -INFINITY : kLn2 * (top + log2f(sum));
         } else {
-#pragma unroll
-          for (int i = 0; i < DP / 8; ++i)
-            *reinterpret_cast<float2*>(dst + (lane >> 2) * DP + i * 8 + (lane & 3) * 2) =
-                make_float2(o[i * 4 + rb * 2], o[i * 4 + rb * 2 + 1]);
+          a.part_o[(int64_t(part) * GT + g) * DP + d] = y;
+          if (d == 0) a.part_ml[int64_t(part) * GT + g] = make_float2(top, sum);
         }
       }
       __syncthreads();
-      if (w == 0) {
-        constexpr int kMine = C::kF32 ? RB : 1;
-#pragma unroll
-        for (int r = 0; r < kMine; ++r) {
-          const int lr = C::kF32 ? r : (lane >> 2), g = rb * RB + lr;
-          float M = -INFINITY, L = 0.f, fac[W];
-#pragma unroll
-          for (int i = 0; i < W; ++i) M = fmaxf(M, ml[i * GT + g].x);
-#pragma unroll
-          for (int i = 0; i < W; ++i) {
-            const float2 x = ml[i * GT + g];
-            fac[i] = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : exp2f(x.x - M);
-            L += x.y * fac[i];
-          }
-          if (g < heads) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            T* out = static_cast<T*>(a.out) + int64_t(c.b) * a.o_row + int64_t(kvh * a.group + g0 + g) * a.o_head;
-            float* po = a.part_o + (int64_t(slot) * GT + g) * DP;
-            const bool one = C::kF32 ? lane == 0 : (lane & 3) == 0;
-            if (one && !whole) a.part_ml[int64_t(slot) * GT + g] = make_float2(M, L);
-            if (one && whole && a.lse)
-              a.lse[int64_t(c.b) * a.kv_heads * a.group + kvh * a.group + g0 + g] =
-                  L == 0.f ? -INFINITY : kLn2 * (M + log2f(L));
-            if constexpr (C::kF32) {
-#pragma unroll
-              for (int i = 0; i < DP / 32; ++i) {
-                const int d = DP == 64 ? lane * 2 + i : (i / 4) * 128 + lane * 4 + (i & 3);
-                float y = o[g * (DP / 32) + i] * fac[0];
-#pragma unroll
-                for (int j = 1; j < W; ++j) y = fmaf(buf[((j - 1) * RB + lr) * DP + d], fac[j], y);
-                if (!whole) po[d] = y;
-                else if (d < a.dim) out[d] = y * inv;
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < DP / 8; ++i) {
-                const int d = i * 8 + (lane & 3) * 2;
-                float y0 = o[i * 4 + rb * 2] * fac[0], y1 = o[i * 4 + rb * 2 + 1] * fac[0];
-#pragma unroll
-                for (int j = 1; j < W; ++j) {
-                  const float2 x = *reinterpret_cast<const float2*>(buf + ((j - 1) * RB + lr) * DP + d);
-                  y0 = fmaf(x.x, fac[j], y0);
-                  y1 = fmaf(x.y, fac[j], y1);
-                }
-                if (!whole) *reinterpret_cast<float2*>(po + d) = make_float2(y0, y1);
-                else if (d < a.dim) {
-                  out[d] = from_f<T>(y0 * inv);
-                  out[d + 1] = from_f<T>(y1 * inv);
-                }
-              }
-            }
-          }
-        }
-      }
     }
   };
 
@@ -559,11 +592,10 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
     cp_async_wait<NS - 1>();
     __syncwarp();
     const int valid = cnt_w[slot];
-    if (valid > 0) step(ring_w + slot * C::kStage, valid, a.group > 8);
+    if (valid > 0) step(ring_w + slot * C::kStage, valid);
     __syncwarp();  // the slot may be refilled
-    slot = slot + 1 == NS ? 0 : slot + 1;
     if (c.tile + 1 == c.ntiles || it + 1 == n) {
-      finish(seg_start, seg_start + c.ntiles);
+      finish(seg_start, seg_start + c.ntiles, slot);
       if (it + 1 < n) {
         seg_start += c.ntiles;
         cursor_next<C::kTile>(c, lens, a.rows, hb);
@@ -573,6 +605,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
     } else {
       ++c.tile;
     }
+    slot = slot + 1 == NS ? 0 : slot + 1;
   }
   cp_async_wait<0>();
 }
@@ -580,9 +613,9 @@ __global__ void __launch_bounds__(Cfg<T, DP_>::W * 32) attend_kernel(const Atten
 // Joins the parts of every (row, head block) that was split, in part order,
 // and writes rows of length 0.  One CTA per row and `per_cta` query heads of a
 // block; its warps take the parts in turn.
-template <typename T, int DP_>
+template <typename T, int DP_, int GT_>
 __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK a, int per_cta) {
-  using C = Cfg<T, DP_>;
+  using C = Cfg<T, DP_, GT_>;
   constexpr int DP = C::DP, GT = C::GT, V = DP / 32;
   __shared__ float s_o[8][DP];
   __shared__ float2 s_ml[8];
@@ -621,8 +654,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK a, int p
         y[i] = z.x, y[i + 1] = z.y;
       }
       const float mn = fmaxf(M, x.x);
-      const float fa = M == -INFINITY ? 0.f : exp2f(M - mn);
-      const float fb = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : exp2f(x.x - mn);
+      const float fa = M == -INFINITY ? 0.f : ex2(M - mn);
+      const float fb = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : ex2(x.x - mn);
       L = L * fa + x.y * fb;
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = acc[i] * fa + y[i] * fb;
@@ -638,7 +671,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK a, int p
     float fac[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      fac[i] = s_ml[i].x == -INFINITY ? (s_ml[i].y != s_ml[i].y ? s_ml[i].y : 0.f) : exp2f(s_ml[i].x - mm);
+      fac[i] = s_ml[i].x == -INFINITY ? (s_ml[i].y != s_ml[i].y ? s_ml[i].y : 0.f) : ex2(s_ml[i].x - mm);
       ll += s_ml[i].y * fac[i];
     }
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
@@ -653,9 +686,9 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const AttendK a, int p
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int GT>
 struct Inst {
-  using C = Cfg<T, DP>;
+  using C = Cfg<T, DP, GT>;
 
   // CTAs of a launch over `rows` rows: all that fit the device at once.  The
   // occupancy is asked for once per device and size class of the row table.
@@ -669,9 +702,9 @@ struct Inst {
     int n = dev < kDevices ? known[cls][dev].load(std::memory_order_acquire) : 0;
     if (n == 0) {
       int occ = 0, sms = 0;
-      SLR_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      SLR_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, DP, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           C::kFixed + kAttendMaxRows * 4));
-      SLR_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, attend_kernel<T, DP>, C::W * 32, *smem));
+      SLR_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, attend_kernel<T, DP, GT>, C::W * 32, *smem));
       SLR_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
       if (occ < 1) return fail(SLR_ERR_UNSUPPORTED, "attend: the kernel does not fit this device");
       n = sms * occ;
@@ -706,6 +739,7 @@ struct Inst {
     a.hblocks = int(ceil_div(a.group, C::GT));
     a.dim = x.dim;
     a.page_size = x.page_size;
+    a.page_shift = (x.page_size & (x.page_size - 1)) == 0 ? __builtin_ctz(x.page_size) : -1;
     a.max_pages = x.max_pages;
     a.num_pages = x.num_pages;
     a.scale_log2 = x.scale * kLog2e;
@@ -729,14 +763,14 @@ struct Inst {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<T, DP>, a));
+    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<T, DP, GT>, a));
     // heads of a block share a joining CTA when there are enough rows to fill the GPU
     const int gt = std::min(C::GT, a.group);
     const int per_cta = int64_t(a.rows) * x.heads <= 8 * 148 ? 1 : gt;
     cfg.gridDim = dim3(a.kv_heads * a.hblocks * int(ceil_div(gt, per_cta)), a.rows);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, DP>, a, per_cta));
+    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, DP, GT>, a, per_cta));
     return SLR_OK;
   }
 
@@ -752,25 +786,37 @@ struct Inst {
   }
 };
 
-template <typename F> int by_shape(int dtype, int dim, F&& f) {
-  const int dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+// Query heads per CTA: the group, rounded up to what the arithmetic offers (8
+// or 16 columns of an MMA; 1, 2, 4 or 8 accumulators per lane in fp32).
+template <typename T, int DP, typename F> int by_group(int group, F&& f) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (group == 1) return f(Inst<T, DP, 1>{});
+    if (group == 2) return f(Inst<T, DP, 2>{});
+    if (group <= 4) return f(Inst<T, DP, 4>{});
+    return f(Inst<T, DP, 8>{});
+  } else {
+    return group <= 8 ? f(Inst<T, DP, 8>{}) : f(Inst<T, DP, 16>{});
+  }
+}
+template <typename T, typename F> int by_dim(int dim, int group, F&& f) {
+  return dim <= 64 ? by_group<T, 64>(group, f) : dim <= 128 ? by_group<T, 128>(group, f) : by_group<T, 256>(group, f);
+}
+template <typename F> int by_shape(int dtype, int dim, int group, F&& f) {
   switch (dtype) {
-    case SLR_F32: return dp == 64 ? f(Inst<float, 64>{}) : dp == 128 ? f(Inst<float, 128>{}) : f(Inst<float, 256>{});
-    case SLR_F16: return dp == 64 ? f(Inst<__half, 64>{}) : dp == 128 ? f(Inst<__half, 128>{}) : f(Inst<__half, 256>{});
-    default:
-      return dp == 64 ? f(Inst<__nv_bfloat16, 64>{})
-                      : dp == 128 ? f(Inst<__nv_bfloat16, 128>{}) : f(Inst<__nv_bfloat16, 256>{});
+    case SLR_F32: return by_dim<float>(dim, group, f);
+    case SLR_F16: return by_dim<__half>(dim, group, f);
+    default: return by_dim<__nv_bfloat16>(dim, group, f);
   }
 }
 
 }  // namespace
 
-int attend_workspace_size(int dtype, int dim, int rows, size_t* bytes) {
-  return by_shape(dtype, dim, [&](auto inst) { return decltype(inst)::size(rows, bytes); });
+int attend_workspace_size(int dtype, int dim, int rows, int group, size_t* bytes) {
+  return by_shape(dtype, dim, group, [&](auto inst) { return decltype(inst)::size(rows, bytes); });
 }
 
 int launch_attend(const AttendArgs& a, cudaStream_t s) {
-  return by_shape(a.dtype, a.dim, [&](auto inst) { return decltype(inst)::launch(a, s); });
+  return by_shape(a.dtype, a.dim, a.heads / a.kv_heads, [&](auto inst) { return decltype(inst)::launch(a, s); });
 }
 
 int read_and_clear_status_attend(unsigned* out) {

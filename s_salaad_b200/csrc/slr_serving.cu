@@ -86,10 +86,14 @@ size_t slr_kv_pages_workspace_size(const slr_kv_cache* cache) {
   return kv_pages_workspace_size(cache->max_rows, cache->num_pages);
 }
 
-size_t slr_kv_attend_workspace_size(const slr_kv_cache* cache) {
+size_t slr_kv_attend_workspace_size(const slr_kv_cache* cache, int32_t rows, int32_t heads) {
   if (check_cache(cache)) return 0;
+  if (rows < 0 || rows > cache->max_rows || heads < 1 || heads % cache->kv_heads) {
+    fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: rows out of range, or heads not a multiple of kv_heads");
+    return 0;
+  }
   size_t n = 0;
-  return attend_workspace_size(cache->dtype, cache->head_dim, cache->max_rows, &n) ? 0 : n;
+  return attend_workspace_size(cache->dtype, cache->head_dim, rows, heads / cache->kv_heads, &n) ? 0 : n;
 }
 
 int slr_kv_advance(const slr_kv_cache* cache, const int32_t* parents, const int32_t* n_new, int32_t n_all,

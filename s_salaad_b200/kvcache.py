@@ -113,7 +113,7 @@ class PagedCache:
         self._pages_ws = int(lib.slr_kv_pages_workspace_size(self._ref))
         if not self._pages_ws:
             raise ValueError(f"PagedCache: {_lib.last_error()}")
-        self._attend_ws: int | None = None
+        self._attend_ws: dict = {}
 
     def _stride(self, i: int) -> int:
         """Stride of pool dimension i; of one of size 1, the packed one."""
@@ -255,12 +255,16 @@ class PagedCache:
                 raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
         lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device) if return_lse else None
         with _DeviceGuard(self.device):
-            if self._attend_ws is None:
-                self._attend_ws = int(self._lib.slr_kv_attend_workspace_size(self._ref))
-            ws = torch.empty(self._attend_ws, dtype=torch.uint8, device=self.device)
+            need = self._attend_ws.get((rows, heads))
+            if need is None:
+                need = int(self._lib.slr_kv_attend_workspace_size(self._ref, rows, heads))
+                if len(self._attend_ws) > 256:
+                    self._attend_ws.clear()
+                self._attend_ws[(rows, heads)] = need
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             rc = self._lib.slr_kv_attend(
                 self._ref, layer, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
                 out.stride(1), _ptr(lse), rows, heads, self.head_dim ** -0.5 if scale is None else scale,
-                ws.data_ptr(), self._attend_ws, _stream(self.device))
+                ws.data_ptr(), need, _stream(self.device))
         _lib.check(rc, "kv_attend")
         return (out, lse) if return_lse else out
