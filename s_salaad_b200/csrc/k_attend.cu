@@ -7,20 +7,20 @@
 // heads of its group only, so the kernel is bound by reading the cache once.
 //
 // Split: the tokens of every (row, block of query heads of one key head)
-// are cut into tiles, all tiles of the call form one list, and each CTA takes
+// are cut into tiles, all tiles of the call form one list, and each warp takes
 // an equal contiguous part of it (computed on the device from lens, so the
 // launch does not depend on the lengths and can be replayed from a graph).
-// A (row, head block) that lies inside one CTA's part is written directly; the
+// A (row, head block) that lies inside one warp's part is written directly; the
 // others leave (o, m, l) per part in the workspace and attend_join_kernel joins
 // them in part order, so results do not depend on timing.
 //
-// Inside a CTA each warp owns a slice of every tile and streams it through
-// its own ring of cp.async stages (no CTA barrier until the end of a row); the
-// page number of a stage is fetched one stage ahead.  Running maximum and sum
-// are per warp and joined through shared memory at the end of a row.
+// A warp streams its tiles through its own ring of cp.async stages, across the
+// ends of rows, and waits for no other warp; the page number of a stage is
+// fetched one stage ahead, the q of the next row (or head block) one row ahead.
 // 16-bit types: Q·Kᵀ and P·V on mma.sync with the query heads of the group as
 // the 16 rows of the MMA (the work is far below tcgen05's tile of 128 rows and
 // the tensor pipe is not the bound).  fp32: FFMA.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -32,6 +32,7 @@ __device__ unsigned g_status_attend;
 
 namespace {
 
+constexpr int kMinTokens = 64;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -46,17 +47,18 @@ struct AttendK {
   void* out;
   int64_t o_row, o_head;
   float* lse;        // [rows, heads] or null
-  float* part_o;     // [2 * ctas][GT][DP]
-  float2* part_ml;   // [2 * ctas][GT]
+  float* part_o;     // [2 * workers][GT][DP]
+  float2* part_ml;   // [2 * workers][GT]
   int32_t* prefix;   // [rows + 1] tiles before each row
-  int rows, kv_heads, group, hblocks, dim, page_size, page_shift, max_pages, num_pages, ctas;
+  int rows, kv_heads, group, hblocks, dim, page_size, page_shift, max_pages, num_pages, workers;
+  int q_pairs, o_pairs;  // q (out) can be read (written) two elements at a time
   float scale_log2;
 };
 
-// Tiles that one CTA takes of a list of n: an equal part, but not less than
+// Tiles that one warp takes of a list of n: an equal part, but not less than
 // min_tiles (a join costs more than a few tiles in a row).
-__device__ __forceinline__ int64_t tiles_per_cta(int64_t n, int ctas, int min_tiles) {
-  const int64_t per = (n + ctas - 1) / ctas;
+__device__ __forceinline__ int64_t tiles_per_worker(int64_t n, int workers, int min_tiles) {
+  const int64_t per = (n + workers - 1) / workers;
   return per < min_tiles ? min_tiles : per;
 }
 
@@ -98,29 +100,24 @@ template <> struct pair_of<__half> {
 };
 
 // Shape of one instance: DP head dimension padded to a power of two, GT query
-// heads per CTA, W warps, TT tokens per warp and tile, NS stages per warp.
-// Two CTAs of 96 KB at DP = 128: 128 KB of loads in flight per SM.
+// heads per warp, W warps, TT tokens per tile, NS stages per warp.  Two CTAs
+// of 96 KB at DP = 128: 128 KB of loads in flight per SM.
 template <typename T, int DP_, int GT_> struct Cfg {
   static constexpr bool kF32 = std::is_same<T, float>::value;
   static constexpr int DP = DP_, GT = GT_;
   static constexpr int W = 4;
   static constexpr int TT = kF32 ? 8 : 16;
-  static constexpr int NS = DP == 64 ? 4 : 3;
-  static constexpr int RB = GT < 8 ? GT : 8;           // heads joined per round at the end of a row
-  static constexpr int kTile = W * TT;
+  static constexpr int NS = kF32 && GT == 8 ? 2 : DP == 64 ? 4 : 3;
   static constexpr int kRow = DP * int(sizeof(T));     // bytes of a token's row
   static constexpr int kHalf = TT * kRow;              // K (or V) bytes of a stage
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kRing = W * NS * kStage;
-  static constexpr int kObuf = DP + 4;                 // floats of a head's row in the join (bank offset 4)
-  static constexpr int kMl = W * GT * 8;
   static constexpr bool kQRegs = GT * DP <= 256;       // fp32: a lane's quarter of q in registers
-  static constexpr int kQ = kF32 && !kQRegs ? GT * DP * 4 : 0;
+  static constexpr int kQ = kF32 && !kQRegs ? W * GT * DP * 4 : 0;
   static constexpr int kP = kF32 ? W * TT * GT * 4 : 0;
   static constexpr int kCnt = W * NS * 4;
-  static constexpr int kFixed = kRing + kMl + kQ + kP + kCnt + 64;
-  static constexpr int kMinTiles = kF32 ? 4 : 2;
-  static_assert(RB * kObuf * 4 <= kStage, "the join's rows take a stage's place");
+  static constexpr int kFixed = kRing + kQ + kP + kCnt + 64;
+  static constexpr int kMinTiles = kMinTokens / TT;
 };
 
 // Place in the list of tiles: row b, head block h, tile of the row.
@@ -128,7 +125,7 @@ struct Cursor {
   int b, h, tile, ntiles, len;
 };
 
-template <int kTile>
+template <int TT>
 __device__ __forceinline__ void cursor_next(Cursor& c, const int* lens, int rows, int hb) {
   if (++c.tile < c.ntiles) return;
   c.tile = 0;
@@ -138,20 +135,26 @@ __device__ __forceinline__ void cursor_next(Cursor& c, const int* lens, int rows
     ++c.b;
   } while (c.b < rows && lens[c.b] == 0);
   c.len = c.b < rows ? lens[c.b] : 0;
-  c.ntiles = (c.len + kTile - 1) / kTile;
+  c.ntiles = (c.len + TT - 1) / TT;
+}
+
+// To the first tile of the next (row, head block).
+template <int TT>
+__device__ __forceinline__ void cursor_skip(Cursor& c, const int* lens, int rows, int hb) {
+  c.tile = c.ntiles - 1;
+  cursor_next<TT>(c, lens, rows, hb);
 }
 
 template <typename T, int DP_, int GT_>
 __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const AttendK a) {
   using C = Cfg<T, DP_, GT_>;
-  constexpr int DP = C::DP, W = C::W, TT = C::TT, NS = C::NS, GT = C::GT, RB = C::RB;
+  constexpr int DP = C::DP, W = C::W, TT = C::TT, NS = C::NS, GT = C::GT;
   constexpr int kThreads = W * 32;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem;
-  float2* ml = reinterpret_cast<float2*>(smem + C::kRing);
-  float* qs = reinterpret_cast<float*>(smem + C::kRing + C::kMl);
-  float* ps = reinterpret_cast<float*>(smem + C::kRing + C::kMl + C::kQ);
-  int* cnt = reinterpret_cast<int*>(smem + C::kRing + C::kMl + C::kQ + C::kP);
+  float* qs = reinterpret_cast<float*>(smem + C::kRing) + (threadIdx.x >> 5) * GT * DP;  // this warp's
+  float* ps = reinterpret_cast<float*>(smem + C::kRing + C::kQ);
+  int* cnt = reinterpret_cast<int*>(smem + C::kRing + C::kQ + C::kP);
   int* scratch = cnt + W * NS;                       // 16 words
   int* lens = reinterpret_cast<int*>(smem + C::kFixed);  // [rows]
 
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   pdl_wait_primary();
   pdl_launch_dependents();
 
-  // ---- this CTA's part of the list of tiles
+  // ---- this warp's part of the list of tiles
   const int64_t cap = int64_t(a.max_pages) * a.page_size;
   const int chunk = (a.rows + kThreads - 1) / kThreads;
   const int r0 = tid * chunk, r1 = min(a.rows, r0 + chunk);
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       n = n < 0 ? 0 : cap;
     }
     lens[r] = int(n);
-    mine += int((n + C::kTile - 1) / C::kTile);
+    mine += int((n + TT - 1) / TT);
   }
   int incl = mine;
 #pragma unroll
@@ -190,15 +193,17 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     total += scratch[i];
   }
   const int64_t n_all = int64_t(total) * hb;
-  const int64_t per = tiles_per_cta(n_all, a.ctas, C::kMinTiles);
-  const int64_t t_begin = int64_t(blockIdx.x) * per;
-  const int64_t t_end = t_begin + per < n_all ? t_begin + per : n_all;
+  const int64_t per = tiles_per_worker(n_all, a.workers, C::kMinTiles);
   for (int r = r0; r < r1; ++r) {
     if (blockIdx.x == 0) a.prefix[r] = before;
-    const int nt = (lens[r] + C::kTile - 1) / C::kTile;
-    if (nt && int64_t(before) * hb <= t_begin && t_begin < int64_t(before + nt) * hb) {
-      scratch[8] = r;
-      scratch[9] = before;
+    const int nt = (lens[r] + TT - 1) / TT;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int64_t t = (int64_t(blockIdx.x) * W + i) * per;
+      if (int64_t(before) * hb <= t && t < int64_t(before + nt) * hb) {
+        scratch[4 + 2 * i] = r;
+        scratch[5 + 2 * i] = before;
+      }
     }
     before += nt;
   }
@@ -207,18 +212,21 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     if (bad) atomicOr(&g_status_attend, SLR_BAD_INDEX_BIT);
   }
   __syncthreads();
-  if (t_begin >= t_end) return;
+  const int worker = int(blockIdx.x) * W + w;
+  const int64_t t_begin = worker * per;
+  const int64_t t_end = t_begin + per < n_all ? t_begin + per : n_all;
+  if (t_begin >= t_end) return;  // no barrier of the CTA from here on
   Cursor c;
-  c.b = scratch[8];
+  c.b = scratch[4 + 2 * w];
   c.len = lens[c.b];
-  c.ntiles = (c.len + C::kTile - 1) / C::kTile;
+  c.ntiles = (c.len + TT - 1) / TT;
   {
-    const int64_t in_row = t_begin - int64_t(scratch[9]) * hb;
+    const int64_t in_row = t_begin - int64_t(scratch[5 + 2 * w]) * hb;
     c.h = int(in_row / c.ntiles);
     c.tile = int(in_row - int64_t(c.h) * c.ntiles);
   }
   const int n = int(t_end - t_begin);
-  // where the first row's tiles start relative to this CTA's part
+  // where the tiles of the current (row, head block) start in the list
   int64_t seg_start = t_begin - c.tile;
 
   // ---- the ring
@@ -230,7 +238,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   auto page_of = [&](int t) { return a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size; };
   Cursor f = c;
   auto fetch_page = [&](const Cursor& u) -> int {
-    const int t0 = u.tile * C::kTile + w * TT;
+    const int t0 = u.tile * TT;
     return t0 < u.len ? a.table[int64_t(u.b) * a.max_pages + page_of(t0)] : 0;
   };
   constexpr int E = 16 / int(sizeof(T));             // elements of a 16-byte chunk
@@ -244,7 +252,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   int loaded = 0, load_slot = 0;
   auto load_stage = [&]() {
     if (loaded < n) {
-      const int t0 = f.tile * C::kTile + w * TT;
+      const int t0 = f.tile * TT;
       int valid = min(TT, f.len - t0);
       if (valid > 0 && (page < 0 || page >= a.num_pages)) {
         if (lane == 0) atomicOr(&g_status_attend, SLR_BAD_INDEX_BIT);
@@ -288,7 +296,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       }
       ++loaded;
       if (loaded < n) {
-        cursor_next<C::kTile>(f, lens, a.rows, hb);
+        cursor_next<TT>(f, lens, a.rows, hb);
         page = fetch_page(f);
       }
       load_slot = load_slot + 1 == NS ? 0 : load_slot + 1;
@@ -307,45 +315,67 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   constexpr int kStat = C::kF32 ? GT : 2 * NT;
   constexpr int kOut = C::kF32 ? GT * (DP / 32) : NT * DP / 4;
   float m[kStat], l[kStat], o[kOut];
-  uint32_t qf[C::kF32 ? 1 : NT * DP / 8];
-  float qr[C::kF32 && C::kQRegs ? GT * DP / 4 : 1];
+  constexpr int kQf = C::kF32 ? 1 : NT * DP / 8, kQr = C::kF32 && C::kQRegs ? GT * DP / 4 : 1;
+  constexpr bool kAhead = C::kF32 ? kQr > 1 && kQr <= 32 : kQf <= 32;  // the next q fits the registers too
+  uint32_t qf[kQf], qf_next[kAhead && !C::kF32 ? kQf : 1];
+  float qr[kQr], qr_next[kAhead && C::kF32 ? kQr : 1];
   auto reset = [&]() {
 #pragma unroll
     for (int i = 0; i < kStat; ++i) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < kOut; ++i) o[i] = 0.f;
   };
-  auto load_q = [&]() {
-    const int kvh = kv_head(c.h), g0 = (c.h - kvh * a.hblocks) * GT;
-    const T* q = static_cast<const T*>(a.q) + int64_t(c.b) * a.q_row + int64_t(kvh * a.group + g0) * a.q_head;
+  // q of the (row, head block) at u into registers (this warp's shared memory for wide fp32 groups)
+  auto load_q = [&](const Cursor& u, uint32_t* to16, float* to32) {
+    const int kvh = kv_head(u.h), g0 = (u.h - kvh * a.hblocks) * GT;
+    const T* q = static_cast<const T*>(a.q) + int64_t(u.b) * a.q_row + int64_t(kvh * a.group + g0) * a.q_head;
     const int heads = min(GT, a.group - g0);
     if constexpr (C::kF32) {
       if constexpr (C::kQRegs) {
 #pragma unroll
-        for (int i = 0; i < GT * DP / 4; ++i) {
+        for (int i = 0; i < kQr; ++i) {
           const int g = i / (DP / 4), d = (lane >> 3) * (DP / 4) + i % (DP / 4);
-          qr[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
+          to32[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
         }
       } else {
-        for (int i = tid; i < GT * DP; i += kThreads) {
+        for (int i = lane; i < GT * DP; i += 32) {
           const int g = i / DP, d = i % DP;
           qs[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
         }
-        __syncthreads();
+        __syncwarp();
       }
     } else {
       const unsigned short* qu = reinterpret_cast<const unsigned short*>(q);
 #pragma unroll
-      for (int i = 0; i < NT * DP / 8; ++i) {
+      for (int i = 0; i < kQf; ++i) {
         // i = (k-step, head tile, half of the k-step)
         const int g = (i >> 1) % NT * 8 + (lane >> 2), d = (i / (2 * NT)) * 16 + (i & 1) * 8 + (lane & 3) * 2;
         uint32_t v = 0;
         if (g < heads && d < a.dim) {
           const unsigned short* p = qu + g * a.q_head + d;
-          v = uint32_t(p[0]) | (uint32_t(p[1]) << 16);
+          v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(p) : uint32_t(p[0]) | (uint32_t(p[1]) << 16);
         }
-        qf[i] = v;
+        to16[i] = v;
       }
+    }
+  };
+  // the q that comes after the one in use, if it is still this warp's
+  auto load_next_q = [&]() {
+    if constexpr (kAhead)
+      if (seg_start + c.ntiles < t_end) {
+        Cursor u = c;
+        cursor_skip<TT>(u, lens, a.rows, hb);
+        load_q(u, qf_next, qr_next);
+      }
+  };
+  auto take_next_q = [&]() {
+    if constexpr (!kAhead) load_q(c, qf, qr);
+    else if constexpr (C::kF32) {
+#pragma unroll
+      for (int i = 0; i < kQr; ++i) qr[i] = qr_next[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kQf; ++i) qf[i] = qf_next[i];
     }
   };
 
@@ -515,77 +545,78 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     }
   };
 
-  // End of a row (or of this CTA's part): the warps' results are joined and
-  // written, final ones as output, parts of a split row to the workspace.
-  // The warps' rows lie in the place of the stage that each has just used.
-  auto finish = [&](int64_t seg0, int64_t seg1, int used) {
+  // End of a row's tiles (or of this warp's part): the result is written as
+  // output, or as one part of a split row to the workspace.
+  auto finish = [&](int64_t seg0, int64_t seg1) {
     const bool whole = seg0 >= t_begin && seg1 <= t_end;
-    const int part = 2 * int(blockIdx.x) + (seg0 >= t_begin ? 1 : 0);
+    const int64_t part = 2 * int64_t(worker) + (seg0 >= t_begin ? 1 : 0);
     const int kvh = kv_head(c.h), g0 = (c.h - kvh * a.hblocks) * GT;
     const int heads = min(GT, a.group - g0);
+    const int64_t head0 = int64_t(kvh) * a.group + g0;
+    T* out = static_cast<T*>(a.out) + int64_t(c.b) * a.o_row + head0 * a.o_head;
+    float* po = a.part_o + part * GT * DP;
     // the sum of a head over the lanes that share it
 #pragma unroll
     for (int i = 0; i < kStat; ++i)
 #pragma unroll
       for (int x = C::kF32 ? 1 : 4; x < (C::kF32 ? 8 : 32); x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
     if constexpr (C::kF32) {
-      if (lane == 0)
 #pragma unroll
-        for (int g = 0; g < GT; ++g) ml[w * GT + g] = make_float2(m[g], l[g]);
-    } else if (lane < 4) {
-#pragma unroll
-      for (int i = 0; i < kStat; ++i) ml[w * GT + (i >> 1) * 8 + lane * 2 + (i & 1)] = make_float2(m[i], l[i]);
-    }
-    float* mine = reinterpret_cast<float*>(ring + (w * NS + used) * C::kStage);
-#pragma unroll
-    for (int rb = 0; rb < GT / RB; ++rb) {
-      if (rb * RB >= heads) break;
-      if constexpr (C::kF32) {
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i)
-            mine[r * C::kObuf + (DP == 64 ? lane * 2 + i : (i / 4) * 128 + lane * 4 + (i & 3))] =
-                o[(rb * RB + r) * (DP / 32) + i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < DP / 4; ++i)
-          mine[((lane & 3) * 2 + (i & 1)) * C::kObuf + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (lane >> 2)] =
-              o[rb * (DP / 4) + i];
-      }
-      __syncthreads();
-      for (int i = tid; i < RB * DP; i += kThreads) {
-        const int lr = i / DP, d = i % DP, g = rb * RB + lr;
+      for (int g = 0; g < GT; ++g) {
+        l[g] = __shfl_sync(0xffffffffu, l[g], 0);
         if (g >= heads) break;
-        float top = -INFINITY, sum = 0.f, y = 0.f;
+        const float inv = l[g] == 0.f ? 0.f : 1.f / l[g];
 #pragma unroll
-        for (int j = 0; j < W; ++j) top = fmaxf(top, ml[j * GT + g].x);
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const float2 x = ml[j * GT + g];
-          // a warp without a finite score has sum 0, or NaN if a score was NaN
-          const float fac = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : ex2(x.x - top);
-          sum = fmaf(x.y, fac, sum);
-          y = fmaf(reinterpret_cast<const float*>(ring + (j * NS + used) * C::kStage)[lr * C::kObuf + d], fac, y);
-        }
-        if (whole) {
-          const int head = kvh * a.group + g0 + g;
-          if (d < a.dim)
-            static_cast<T*>(a.out)[int64_t(c.b) * a.o_row + int64_t(head) * a.o_head + d] =
-                from_f<T>(sum == 0.f ? 0.f : y / sum);
-          if (d == 0 && a.lse)
-            a.lse[int64_t(c.b) * a.kv_heads * a.group + head] = sum == 0.f ? -INFINITY : kLn2 * (top + log2f(sum));
-        } else {
-          a.part_o[(int64_t(part) * GT + g) * DP + d] = y;
-          if (d == 0) a.part_ml[int64_t(part) * GT + g] = make_float2(top, sum);
+        for (int i = 0; i < DP / 32; ++i) {
+          const int d = DP == 64 ? lane * 2 + i : (i / 4) * 128 + lane * 4 + (i & 3);
+          const float y = o[g * (DP / 32) + i];
+          if (!whole) po[g * DP + d] = y;
+          else if (d < a.dim) out[g * a.o_head + d] = y * inv;
         }
       }
-      __syncthreads();
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (nt * 8 >= heads) break;
+        const float inv0 = l[nt * 2] == 0.f ? 0.f : 1.f / l[nt * 2];
+        const float inv1 = l[nt * 2 + 1] == 0.f ? 0.f : 1.f / l[nt * 2 + 1];
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+          const float y0 = o[nt * (DP / 4) + i * 2], y1 = o[nt * (DP / 4) + i * 2 + 1];
+          if (whole) {
+            // heads across lanes, two columns in each
+            const uint32_t v = transpose8(pair_of<T>::pack(y0 * inv0, y1 * inv1));
+            const int g = nt * 8 + (lane >> 2), d = i * 8 + (lane & 3) * 2;
+            if (g < heads && d < a.dim) {
+              unsigned short* dst = reinterpret_cast<unsigned short*>(out) + g * a.o_head + d;
+              if (a.o_pairs) *reinterpret_cast<uint32_t*>(dst) = v;
+              else dst[0] = static_cast<unsigned short>(v), dst[1] = static_cast<unsigned short>(v >> 16);
+            }
+          } else {
+            float* dst = po + (nt * 8 + (lane & 3) * 2) * DP + i * 8 + (lane >> 2);
+            if (nt * 8 + (lane & 3) * 2 < heads) dst[0] = y0;
+            if (nt * 8 + (lane & 3) * 2 + 1 < heads) dst[DP] = y1;
+          }
+        }
+      }
+    }
+    // one lane per head: its maximum and sum
+    if (C::kF32 ? lane == 0 : lane < 4) {
+#pragma unroll
+      for (int i = 0; i < kStat; ++i) {
+        const int g = C::kF32 ? i : (i >> 1) * 8 + lane * 2 + (i & 1);
+        if (g >= heads) continue;
+        if (!whole) a.part_ml[part * GT + g] = make_float2(m[i], l[i]);
+        else if (a.lse)
+          a.lse[int64_t(c.b) * a.kv_heads * a.group + head0 + g] =
+              l[i] == 0.f ? -INFINITY : kLn2 * ((m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i]));
+      }
     }
   };
 
   reset();
-  load_q();
+  load_q(c, qf, qr);
+  load_next_q();
   int slot = 0;
   for (int it = 0; it < n; ++it) {
     load_stage();
@@ -595,12 +626,13 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     if (valid > 0) step(ring_w + slot * C::kStage, valid);
     __syncwarp();  // the slot may be refilled
     if (c.tile + 1 == c.ntiles || it + 1 == n) {
-      finish(seg_start, seg_start + c.ntiles, slot);
+      finish(seg_start, seg_start + c.ntiles);
       if (it + 1 < n) {
         seg_start += c.ntiles;
-        cursor_next<C::kTile>(c, lens, a.rows, hb);
+        cursor_next<TT>(c, lens, a.rows, hb);
         reset();
-        load_q();
+        take_next_q();
+        load_next_q();
       }
     } else {
       ++c.tile;
@@ -610,80 +642,82 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   cp_async_wait<0>();
 }
 
-// Joins the parts of every (row, head block) that was split, in part order,
-// and writes rows of length 0.  One CTA per row and `per_cta` query heads of a
-// block; its warps take the parts in turn.
+// Joins the parts of every (row, head) that was split, in part order, and
+// writes rows of length 0.  `wph` warps (a power of two) share a head: each
+// joins every wph-th part, then the first joins theirs.
 template <typename T, int DP_, int GT_>
-__global__ void __launch_bounds__(256) attend_join_kernel(const AttendK a, int per_cta) {
+__global__ void __launch_bounds__(1024) attend_join_kernel(const AttendK a, int wph) {
   using C = Cfg<T, DP_, GT_>;
   constexpr int DP = C::DP, GT = C::GT, V = DP / 32;
-  __shared__ float s_o[8][DP];
-  __shared__ float2 s_ml[8];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hb = a.kv_heads * a.hblocks;
-  const int groups = (min(GT, a.group) + per_cta - 1) / per_cta;
-  const int h = blockIdx.x / groups, g_first = (blockIdx.x % groups) * per_cta, b = blockIdx.y;
-  const int kvh = h / a.hblocks, g0 = (h % a.hblocks) * GT;
-  const int heads = min(GT, a.group - g0);
+  __shared__ float s_o[32][DP];
+  __shared__ float2 s_ml[32];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int hb = a.kv_heads * a.hblocks, n_heads = a.kv_heads * a.group;
+  const int64_t item = int64_t(blockIdx.x) * (warps / wph) + w / wph;  // (row, head)
+  const int sub = w % wph;
+  const bool in = item < int64_t(a.rows) * n_heads;
+  const int b = in ? int(item / n_heads) : 0, head = in ? int(item % n_heads) : 0;
+  const int kvh = head / a.group, hg = head % a.group, h = kvh * a.hblocks + hg / GT, g = hg % GT;
   pdl_wait_primary();
   const int p0 = a.prefix[b], p1 = a.prefix[b + 1];
-  const int64_t per = tiles_per_cta(int64_t(a.prefix[a.rows]) * hb, a.ctas, C::kMinTiles);
-  const int tiles = p1 - p0;
+  const int64_t per = tiles_per_worker(int64_t(a.prefix[a.rows]) * hb, a.workers, C::kMinTiles);
+  const int tiles = in ? p1 - p0 : 0;
   const int64_t t0 = int64_t(p0) * hb + int64_t(h) * tiles, t1 = t0 + tiles;
   const int c0 = tiles ? int(t0 / per) : 0, c1 = tiles ? int((t1 - 1) / per) : 0;
-  if (tiles && c0 == c1) return;
-  for (int g = g_first; g < min(heads, g_first + per_cta); ++g) {
-    const int head = kvh * a.group + g0 + g;
-    T* out = static_cast<T*>(a.out) + int64_t(b) * a.o_row + int64_t(head) * a.o_head;
-    float* lse = a.lse ? a.lse + int64_t(b) * a.kv_heads * a.group + head : nullptr;
-    if (!tiles) {
-      for (int d = threadIdx.x; d < a.dim; d += blockDim.x) out[d] = from_f<T>(0.f);
-      if (lse && threadIdx.x == 0) *lse = -INFINITY;
-      continue;
-    }
-    float M = -INFINITY, L = 0.f, acc[V] = {};
-#pragma unroll 4
-    for (int c = c0 + w; c <= c1; c += 8) {
-      const int64_t slot = 2 * int64_t(c) + (c == c0 ? 1 : 0);
-      const float2 x = a.part_ml[slot * GT + g];
-      const float* src = a.part_o + (slot * GT + g) * DP + lane * V;
-      float y[V];
+  const bool split = c0 != c1;
+  float M = -INFINITY, L = 0.f, acc[V] = {};
+  auto add = [&](const float2 x, const float* y) {
+    const float mn = fmaxf(M, x.x);
+    const float fa = M == -INFINITY ? 0.f : ex2(M - mn);
+    // a part without a finite score has sum 0, or NaN if a score was NaN
+    const float fb = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : ex2(x.x - mn);
+    L = L * fa + x.y * fb;
 #pragma unroll
-      for (int i = 0; i < V; i += 2) {
-        const float2 z = *reinterpret_cast<const float2*>(src + i);
-        y[i] = z.x, y[i + 1] = z.y;
-      }
-      const float mn = fmaxf(M, x.x);
-      const float fa = M == -INFINITY ? 0.f : ex2(M - mn);
-      const float fb = x.x == -INFINITY ? (x.y != x.y ? x.y : 0.f) : ex2(x.x - mn);
-      L = L * fa + x.y * fb;
+    for (int i = 0; i < V; ++i) acc[i] = acc[i] * fa + y[i] * fb;
+    M = mn;
+  };
+  if (split) {
+    constexpr int U = 4;
+    for (int c = c0 + sub; c <= c1; c += U * wph) {
+      float2 x[U];
+      float y[U][V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] = acc[i] * fa + y[i] * fb;
-      M = mn;
+      for (int u = 0; u < U; ++u)
+        if (c + u * wph <= c1) {
+          const int64_t slot = 2 * int64_t(c + u * wph) + (c + u * wph == c0 ? 1 : 0);
+          x[u] = a.part_ml[slot * GT + g];
+          const float* src = a.part_o + (slot * GT + g) * DP + lane * V;
+#pragma unroll
+          for (int i = 0; i < V; i += 2) {
+            const float2 z = *reinterpret_cast<const float2*>(src + i);
+            y[u][i] = z.x, y[u][i + 1] = z.y;
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c + u * wph <= c1) add(x[u], y[u]);
     }
+  }
+  if (wph > 1) {
     if (lane == 0) s_ml[w] = make_float2(M, L);
 #pragma unroll
     for (int i = 0; i < V; ++i) s_o[w][lane * V + i] = acc[i];
     __syncthreads();
-    float mm = -INFINITY, ll = 0.f;
+    if (sub) return;
+    for (int i = 1; i < wph; ++i) {
+      float y[V];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mm = fmaxf(mm, s_ml[i].x);
-    float fac[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      fac[i] = s_ml[i].x == -INFINITY ? (s_ml[i].y != s_ml[i].y ? s_ml[i].y : 0.f) : ex2(s_ml[i].x - mm);
-      ll += s_ml[i].y * fac[i];
+      for (int j = 0; j < V; ++j) y[j] = s_o[w + i][lane * V + j];
+      add(s_ml[w + i], y);
     }
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    for (int d = threadIdx.x; d < a.dim; d += blockDim.x) {
-      float y = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y = fmaf(s_o[i][d], fac[i], y);
-      out[d] = from_f<T>(y * inv);
-    }
-    if (lse && threadIdx.x == 0) *lse = ll == 0.f ? -INFINITY : kLn2 * (mm + log2f(ll));
-    __syncthreads();
   }
+  if (!in || (tiles && !split)) return;
+  T* out = static_cast<T*>(a.out) + int64_t(b) * a.o_row + int64_t(head) * a.o_head + lane * V;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (lane * V + i < a.dim) out[i] = from_f<T>(L == 0.f ? 0.f : acc[i] / L);
+  if (lane == 0 && a.lse)
+    a.lse[int64_t(b) * n_heads + head] = L == 0.f ? -INFINITY : kLn2 * ((M == -INFINITY ? 0.f : M) + log2f(L));
 }
 
 template <typename T, int DP, int GT>
@@ -692,7 +726,7 @@ struct Inst {
 
   // CTAs of a launch over `rows` rows: all that fit the device at once.  The
   // occupancy is asked for once per device and size class of the row table.
-  static int prepare(int rows, size_t* smem, int* ctas) {
+  static int prepare(int rows, size_t* smem, int* workers) {
     constexpr int kDevices = 32;
     static std::atomic<int> known[2][kDevices];
     const int cls = rows <= 256 ? 0 : 1;
@@ -710,14 +744,14 @@ struct Inst {
       n = sms * occ;
       if (dev < kDevices) known[cls][dev].store(n, std::memory_order_release);
     }
-    *ctas = n;
+    *workers = n * C::W;
     return SLR_OK;
   }
 
   static int launch(const AttendArgs& x, cudaStream_t s) {
     AttendK a = {};
     size_t smem = 0;
-    int rc = prepare(x.rows, &smem, &a.ctas);
+    int rc = prepare(x.rows, &smem, &a.workers);
     if (rc) return rc;
     a.k = x.k;
     a.v = x.v;
@@ -743,45 +777,50 @@ struct Inst {
     a.max_pages = x.max_pages;
     a.num_pages = x.num_pages;
     a.scale_log2 = x.scale * kLog2e;
-    // no more CTAs than tiles that rows of the greatest length could have
+    a.q_pairs = a.q_row % 2 == 0 && a.q_head % 2 == 0 && reinterpret_cast<uintptr_t>(a.q) % 4 == 0;
+    a.o_pairs = a.o_row % 2 == 0 && a.o_head % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % 4 == 0;
+    // no more warps than shares of tiles that rows of the greatest length could have
     const int64_t most = int64_t(a.rows) * a.kv_heads * a.hblocks *
-                         ceil_div(int64_t(a.max_pages) * a.page_size, C::kTile * C::kMinTiles);
-    if (most < a.ctas) a.ctas = int(most < 1 ? 1 : most);
+                         ceil_div(int64_t(a.max_pages) * a.page_size, int64_t(C::TT) * C::kMinTiles);
+    if (most < a.workers) a.workers = int(round_up(most, C::W));
     uint8_t* ws = static_cast<uint8_t*>(x.workspace);
     a.part_o = reinterpret_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float2*>(ws + size_t(2 * a.ctas) * C::GT * DP * 4);
-    a.prefix = reinterpret_cast<int32_t*>(ws + size_t(2 * a.ctas) * C::GT * (DP * 4 + 8));
-    if (need(a.ctas, a.rows) > x.workspace_bytes)
-      return fail(SLR_ERR_WORKSPACE, "attend: workspace too small, need " + std::to_string(need(a.ctas, a.rows)) + " bytes");
+    a.part_ml = reinterpret_cast<float2*>(ws + size_t(2 * a.workers) * C::GT * DP * 4);
+    a.prefix = reinterpret_cast<int32_t*>(ws + size_t(2 * a.workers) * C::GT * (DP * 4 + 8));
+    if (need(a.workers, a.rows) > x.workspace_bytes)
+      return fail(SLR_ERR_WORKSPACE,
+                  "attend: workspace too small, need " + std::to_string(need(a.workers, a.rows)) + " bytes");
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.ctas);
+    cfg.gridDim = dim3(a.workers / C::W);
     cfg.blockDim = dim3(C::W * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<T, DP, GT>, a));
-    // heads of a block share a joining CTA when there are enough rows to fill the GPU
-    const int gt = std::min(C::GT, a.group);
-    const int per_cta = int64_t(a.rows) * x.heads <= 8 * 148 ? 1 : gt;
-    cfg.gridDim = dim3(a.kv_heads * a.hblocks * int(ceil_div(gt, per_cta)), a.rows);
-    cfg.blockDim = dim3(256);
+    // warps per head of the join: a fourth of the parts that an even split of
+    // the longest possible rows gives each (they are read four at a time)
+    int wph = 1;
+    while (wph < 32 && int64_t(wph) * 4 * a.rows * a.kv_heads * a.hblocks < a.workers) wph *= 2;
+    const int warps = std::max(wph, 8);
+    cfg.gridDim = dim3(unsigned(ceil_div(int64_t(a.rows) * x.heads, warps / wph)));
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = 0;
-    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, DP, GT>, a, per_cta));
+    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_join_kernel<T, DP, GT>, a, wph));
     return SLR_OK;
   }
 
-  static size_t need(int ctas, int rows) {
-    return size_t(2 * ctas) * C::GT * (DP * 4 + 8) + size_t(rows + 1) * 4;
+  static size_t need(int workers, int rows) {
+    return size_t(2 * workers) * C::GT * (DP * 4 + 8) + size_t(rows + 1) * 4;
   }
   static int size(int rows, size_t* out) {
     size_t smem = 0;
-    int ctas = 0;
-    int rc = prepare(rows, &smem, &ctas);
-    *out = rc ? 0 : need(ctas, rows);
+    int workers = 0;
+    int rc = prepare(rows, &smem, &workers);
+    *out = rc ? 0 : need(workers, rows);
     return rc;
   }
 };
