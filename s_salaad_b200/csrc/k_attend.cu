@@ -7,8 +7,9 @@
 // heads of its group only, so the kernel is bound by reading the cache once.
 //
 // Split: the tokens of every (row, block of query heads of one key head)
-// are cut into tiles, all tiles of the call form one list, and each warp takes
-// an equal contiguous part of it (computed on the device from lens, so the
+// are cut into tiles, all tiles of the call form one list (with kEndCost empty
+// places behind each row's: the end of a row costs about as much time as that
+// many tiles), and each warp takes an equal contiguous part of it (computed on the device from lens, so the
 // launch does not depend on the lengths and can be replayed from a graph).
 // A (row, head block) that lies inside one warp's part is written directly; the
 // others leave (o, m, l) per part in the workspace and attend_join_kernel joins
@@ -49,13 +50,18 @@ struct AttendK {
   float* lse;        // [rows, heads] or null
   float* part_o;     // [2 * workers][GT][DP]
   float2* part_ml;   // [2 * workers][GT]
-  int32_t* prefix;   // [rows + 1] tiles before each row
+  int32_t* prefix;   // [rows + 1] places before each row
   int rows, kv_heads, group, hblocks, dim, page_size, page_shift, max_pages, num_pages, workers;
-  int q_pairs, o_pairs;  // q (out) can be read (written) two elements at a time
+  int q_wide, o_pairs;  // q can be read in 16 bytes (fp32) or two elements, out written in two elements
   float scale_log2;
 };
 
-// Tiles that one warp takes of a list of n: an equal part, but not less than
+// Without it a warp whose part was 28 rows of one token took 1.8 times as long
+// as the others (8 rows of 1 to 2050 tokens, 32 heads, fp32: 77 us).
+constexpr int kEndCost = 1;
+__device__ __forceinline__ int places(int tiles) { return tiles ? tiles + kEndCost : 0; }
+
+// Places that one warp takes of a list of n: an equal part, but not less than
 // min_tiles (a join costs more than a few tiles in a row).
 __device__ __forceinline__ int64_t tiles_per_worker(int64_t n, int workers, int min_tiles) {
   const int64_t per = (n + workers - 1) / workers;
@@ -123,12 +129,15 @@ template <typename T, int DP_, int GT_> struct Cfg {
 // Place in the list of tiles: row b, head block h, tile of the row.
 struct Cursor {
   int b, h, tile, ntiles, len;
+  int64_t seg;  // place of its first tile
+  __device__ int64_t place() const { return seg + tile; }
 };
 
 template <int TT>
 __device__ __forceinline__ void cursor_next(Cursor& c, const int* lens, int rows, int hb) {
   if (++c.tile < c.ntiles) return;
   c.tile = 0;
+  c.seg += places(c.ntiles);
   if (++c.h < hb) return;
   c.h = 0;
   do {
@@ -176,7 +185,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       n = n < 0 ? 0 : cap;
     }
     lens[r] = int(n);
-    mine += int((n + TT - 1) / TT);
+    mine += places(int((n + TT - 1) / TT));
   }
   int incl = mine;
 #pragma unroll
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   const int64_t per = tiles_per_worker(n_all, a.workers, C::kMinTiles);
   for (int r = r0; r < r1; ++r) {
     if (blockIdx.x == 0) a.prefix[r] = before;
-    const int nt = (lens[r] + TT - 1) / TT;
+    const int nt = places((lens[r] + TT - 1) / TT);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const int64_t t = (int64_t(blockIdx.x) * W + i) * per;
@@ -221,13 +230,14 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   c.len = lens[c.b];
   c.ntiles = (c.len + TT - 1) / TT;
   {
-    const int64_t in_row = t_begin - int64_t(scratch[5 + 2 * w]) * hb;
-    c.h = int(in_row / c.ntiles);
-    c.tile = int(in_row - int64_t(c.h) * c.ntiles);
+    const int64_t row0 = int64_t(scratch[5 + 2 * w]) * hb, per_head = places(c.ntiles);
+    c.h = int((t_begin - row0) / per_head);
+    c.seg = row0 + c.h * per_head;
+    c.tile = int(t_begin - c.seg);
+    // between two rows: on to the next
+    if (c.tile >= c.ntiles) cursor_skip<TT>(c, lens, a.rows, hb);
   }
-  const int n = int(t_end - t_begin);
-  // where the tiles of the current (row, head block) start in the list
-  int64_t seg_start = t_begin - c.tile;
+  if (c.place() >= t_end || c.b >= a.rows) return;
 
   // ---- the ring
   // Chunk `ch` of a token's row lies at ch ^ (row & 7): the eight rows of an
@@ -248,10 +258,22 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   const int lrow = lane / CH, lch = lane % CH;
   const uint32_t ldst = lrow * C::kRow + ((lch ^ lrow) << 4);
   const int64_t lsrc = lrow * a.token_stride + lch * E;
+  // one lane per 128 bytes of a block's q
+  auto prefetch_q = [&]() {
+    constexpr int kLine = 128 / int(sizeof(T)), kLines = DP / kLine;
+    const int kvh = kv_head(f.h), g0 = (f.h - kvh * a.hblocks) * GT;
+    const T* q = static_cast<const T*>(a.q) + int64_t(f.b) * a.q_row + int64_t(kvh * a.group + g0) * a.q_head;
+#pragma unroll
+    for (int i = 0; i < GT * kLines; i += 32) {
+      const int g = (i + lane) / kLines, d = (i + lane) % kLines * kLine;
+      if (g < GT && g0 + g < a.group && d < a.dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + g * a.q_head + d));
+    }
+  };
   int page = fetch_page(f);
-  int loaded = 0, load_slot = 0;
+  int load_slot = 0;
+  bool more = true;  // tiles left to load
   auto load_stage = [&]() {
-    if (loaded < n) {
+    if (more) {
       const int t0 = f.tile * TT;
       int valid = min(TT, f.len - t0);
       if (valid > 0 && (page < 0 || page >= a.num_pages)) {
@@ -294,10 +316,11 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
           }
         }
       }
-      ++loaded;
-      if (loaded < n) {
-        cursor_next<TT>(f, lens, a.rows, hb);
+      cursor_next<TT>(f, lens, a.rows, hb);
+      more = f.b < a.rows && f.place() < t_end;
+      if (more) {
         page = fetch_page(f);
+        if (f.tile == 0) prefetch_q();
       }
       load_slot = load_slot + 1 == NS ? 0 : load_slot + 1;
     }
@@ -333,9 +356,14 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     if constexpr (C::kF32) {
       if constexpr (C::kQRegs) {
 #pragma unroll
-        for (int i = 0; i < kQr; ++i) {
+        for (int i = 0; i < kQr; i += 4) {
           const int g = i / (DP / 4), d = (lane >> 3) * (DP / 4) + i % (DP / 4);
-          to32[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (g < heads && d < a.dim) {  // head_dim is a multiple of 8
+            const float* p = q + g * a.q_head + d;
+            v = a.q_wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+          }
+          to32[i] = v.x, to32[i + 1] = v.y, to32[i + 2] = v.z, to32[i + 3] = v.w;
         }
       } else {
         for (int i = lane; i < GT * DP; i += 32) {
@@ -353,7 +381,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
         uint32_t v = 0;
         if (g < heads && d < a.dim) {
           const unsigned short* p = qu + g * a.q_head + d;
-          v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(p) : uint32_t(p[0]) | (uint32_t(p[1]) << 16);
+          v = a.q_wide ? *reinterpret_cast<const uint32_t*>(p) : uint32_t(p[0]) | (uint32_t(p[1]) << 16);
         }
         to16[i] = v;
       }
@@ -362,10 +390,10 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   // the q that comes after the one in use, if it is still this warp's
   auto load_next_q = [&]() {
     if constexpr (kAhead)
-      if (seg_start + c.ntiles < t_end) {
+      if (c.seg + places(c.ntiles) < t_end) {
         Cursor u = c;
         cursor_skip<TT>(u, lens, a.rows, hb);
-        load_q(u, qf_next, qr_next);
+        if (u.b < a.rows) load_q(u, qf_next, qr_next);
       }
   };
   auto take_next_q = [&]() {
@@ -618,26 +646,24 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   load_q(c, qf, qr);
   load_next_q();
   int slot = 0;
-  for (int it = 0; it < n; ++it) {
+  while (true) {
     load_stage();
     cp_async_wait<NS - 1>();
     __syncwarp();
     const int valid = cnt_w[slot];
     if (valid > 0) step(ring_w + slot * C::kStage, valid);
     __syncwarp();  // the slot may be refilled
-    if (c.tile + 1 == c.ntiles || it + 1 == n) {
-      finish(seg_start, seg_start + c.ntiles);
-      if (it + 1 < n) {
-        seg_start += c.ntiles;
-        cursor_next<TT>(c, lens, a.rows, hb);
-        reset();
-        take_next_q();
-        load_next_q();
-      }
-    } else {
-      ++c.tile;
-    }
     slot = slot + 1 == NS ? 0 : slot + 1;
+    if (c.tile + 1 < c.ntiles && c.place() + 1 < t_end) {
+      ++c.tile;
+      continue;
+    }
+    finish(c.seg, c.seg + c.ntiles);
+    cursor_skip<TT>(c, lens, a.rows, hb);
+    if (c.b >= a.rows || c.place() >= t_end) break;
+    reset();
+    take_next_q();
+    load_next_q();
   }
   cp_async_wait<0>();
 }
@@ -661,8 +687,8 @@ __global__ void __launch_bounds__(1024) attend_join_kernel(const AttendK a, int 
   pdl_wait_primary();
   const int p0 = a.prefix[b], p1 = a.prefix[b + 1];
   const int64_t per = tiles_per_worker(int64_t(a.prefix[a.rows]) * hb, a.workers, C::kMinTiles);
-  const int tiles = in ? p1 - p0 : 0;
-  const int64_t t0 = int64_t(p0) * hb + int64_t(h) * tiles, t1 = t0 + tiles;
+  const int tiles = in && p1 > p0 ? p1 - p0 - kEndCost : 0;
+  const int64_t t0 = int64_t(p0) * hb + int64_t(h) * places(tiles), t1 = t0 + tiles;
   const int c0 = tiles ? int(t0 / per) : 0, c1 = tiles ? int((t1 - 1) / per) : 0;
   const bool split = c0 != c1;
   float M = -INFINITY, L = 0.f, acc[V] = {};
@@ -777,7 +803,8 @@ struct Inst {
     a.max_pages = x.max_pages;
     a.num_pages = x.num_pages;
     a.scale_log2 = x.scale * kLog2e;
-    a.q_pairs = a.q_row % 2 == 0 && a.q_head % 2 == 0 && reinterpret_cast<uintptr_t>(a.q) % 4 == 0;
+    const int64_t kw = C::kF32 ? 4 : 2;
+    a.q_wide = a.q_row % kw == 0 && a.q_head % kw == 0 && reinterpret_cast<uintptr_t>(a.q) % (kw * sizeof(T)) == 0;
     a.o_pairs = a.o_row % 2 == 0 && a.o_head % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % 4 == 0;
     // no more warps than shares of tiles that rows of the greatest length could have
     const int64_t most = int64_t(a.rows) * a.kv_heads * a.hblocks *
