@@ -56,9 +56,10 @@ struct AttendK {
   float scale_log2;
 };
 
-// Without it a warp whose part was 28 rows of one token took 1.8 times as long
-// as the others (8 rows of 1 to 2050 tokens, 32 heads, fp32: 77 us).
-constexpr int kEndCost = 1;
+// A row's end (its output, the next row's q from DRAM) takes the time of some
+// tiles.  8 rows of 1 to 4100 tokens, 32 heads, bf16: 1 place 77 us, 2: 58, 3:
+// 52.5, 4: 52.7, 6: 53; 400 rows of 1 to 700 tokens: 129, 118, 109.5, 113, 111.
+constexpr int kEndCost = 3;
 __device__ __forceinline__ int places(int tiles) { return tiles ? tiles + kEndCost : 0; }
 
 // Places that one warp takes of a list of n: an equal part, but not less than

@@ -3,12 +3,16 @@
 //
 //   lse = log Σ_j e^x_j,   logprob = x_target - lse,   H = lse - Σ_j p_j x_j
 //
-// Bound by reading the logits once (16-bit types: close to the exp2 rate too).
-// Each thread streams 16-byte vectors and keeps a running maximum m and the
-// sums s = Σ 2^t and u = Σ t 2^t with t = (x - m)·log2 e; the triples join
-// associatively: over a thread's batches, a block and a cluster of CTAs that
-// share a row (few rows: up to 8 CTAs per row through distributed shared
-// memory, one launch, no workspace; many rows: one CTA per row).
+// Bound by reading the logits once (16-bit types: the exp2 rate, 16 per clock
+// and SM, is close behind).  Each thread streams 16-byte vectors and keeps a
+// running maximum m and the sums s = Σ 2^t and u = Σ t 2^t with
+// t = (x - m)·log2 e; the triples join associatively: over a thread's batches,
+// a block and a cluster of CTAs that share a row (few rows: up to 8 CTAs per
+// row through distributed shared memory, one launch, no workspace; many rows:
+// one CTA per row).  About 6 instructions per element: t is one multiply-add,
+// and -inf is raised to a finite value so that it adds 0 to u; where that is
+// not exact (a part whose greatest logit is -inf or of the order of the type's
+// lowest or greatest value) the part is summed again element by element.
 //
 // The k best need no second pass over the row: each thread also keeps its
 // greatest value and the vector that held it.  The k-th greatest of these
@@ -96,54 +100,75 @@ __device__ __forceinline__ Key warp_merge(Key a, Key b_reversed) {
   return k;
 }
 
-template <typename T> struct Vec {
-  static constexpr int E = 16 / int(sizeof(T));
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int E = 4;
+  static constexpr float kClip = -1e38f;  // stands for anything below
+  static constexpr float kLow = -1e37f, kHigh = 1e37f;
   __device__ static void to_floats(const uint4& v, float* f) {
-    if constexpr (std::is_same<T, float>::value) {
-      f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
-    } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+  __device__ static void clipped(const uint4& v, float* f) {
+    to_floats(v, f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 p;
-        if constexpr (std::is_same<T, __half>::value) p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        else p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-        f[2 * i] = p.x, f[2 * i + 1] = p.y;
-      }
-    }
+    for (int i = 0; i < 4; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(f[i]) : "f"(kClip));  // NaN stays
   }
   // the greatest element; NaN is passed over
-  __device__ static float greatest(const uint4& v) {
-    if constexpr (std::is_same<T, float>::value) {
-      return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
-    } else {
-      using P = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-      const P a = *reinterpret_cast<const P*>(&v.x), b = *reinterpret_cast<const P*>(&v.y);
-      const P c = *reinterpret_cast<const P*>(&v.z), d = *reinterpret_cast<const P*>(&v.w);
-      const P m = __hmax2(__hmax2(a, b), __hmax2(c, d));
-      return fmaxf(to_f(m.x), to_f(m.y));
-    }
+  using Top = float;
+  __device__ static Top top(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
+  __device__ static Top greater(Top a, Top b) { return fmaxf(a, b); }
+  __device__ static float of_top(Top a) { return a; }
+};
+template <typename T, typename P> struct Vec16 {
+  static constexpr int E = 8;
+  __device__ static P as(uint32_t w) { return *reinterpret_cast<P*>(&w); }
+  __device__ static void unpack(const P* p, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = to_f(p[i].x), f[2 * i + 1] = to_f(p[i].y);
+  }
+  __device__ static void to_floats(const uint4& v, float* f) {
+    const P p[4] = {as(v.x), as(v.y), as(v.z), as(v.w)};
+    unpack(p, f);
+  }
+  __device__ static void clipped(const uint4& v, float* f) {
+    const P low = {from_f<T>(Vec<T>::kClip), from_f<T>(Vec<T>::kClip)};
+    const P p[4] = {__hmax2_nan(as(v.x), low), __hmax2_nan(as(v.y), low), __hmax2_nan(as(v.z), low),
+                    __hmax2_nan(as(v.w), low)};
+    unpack(p, f);
+  }
+  using Top = P;
+  __device__ static Top top(const uint4& v) {
+    return __hmax2(__hmax2(as(v.x), as(v.y)), __hmax2(as(v.z), as(v.w)));
+  }
+  __device__ static Top greater(Top a, Top b) { return __hmax2(a, b); }
+  __device__ static float of_top(Top a) { return fmaxf(to_f(a.x), to_f(a.y)); }
+};
+template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
+  static constexpr float kClip = -1e38f, kLow = -1e37f, kHigh = 1e37f;
+};
+template <> struct Vec<__half> : Vec16<__half, __half2> {
+  static constexpr float kClip = -65504.f, kLow = -6e4f, kHigh = 1e37f;
 };
 
-// A row as 16-byte vectors on 16-byte boundaries: vector j holds elements
-// [j * E - shift, j * E - shift + E), of which those outside [0, vocab) do
-// not exist (only the first and the last vector can have such).
+// A row as the 16-byte vectors on 16-byte boundaries inside it (vector j:
+// elements [head + j E, head + j E + E)) and up to 2 (E - 1) elements at its
+// ends.
 template <typename T> struct Row {
   static constexpr int E = Vec<T>::E;
   const T* x;
-  int64_t vocab;
-  int shift;
-  __device__ uint4 load(int64_t j) const {
-    const int64_t i = j * E - shift;
-    if (i >= 0 && i + E <= vocab) return __ldg(reinterpret_cast<const uint4*>(x + i));
-    T t[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) t[e] = i + e >= 0 && i + e < vocab ? x[i + e] : from_f<T>(-INFINITY);
-    uint4 v;
-    memcpy(&v, t, 16);
-    return v;
+  int head, vectors, edges;
+  __device__ Row(const T* p, int vocab) : x(p) {
+    const int shift = int((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+    head = min(vocab, (E - shift) % E);
+    vectors = (vocab - head) / E;
+    edges = vocab - vectors * E;
   }
+  __device__ uint4 load(int j) const { return __ldg(reinterpret_cast<const uint4*>(x + head) + j); }
+  __device__ int first_of(int j) const { return head + j * E; }
+  // element index of edge e < edges
+  __device__ int edge(int e) const { return e < head ? e : e + vectors * E; }
 };
 
 struct Shared {
@@ -159,90 +184,137 @@ struct Shared {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a) {
-  constexpr int E = Vec<T>::E;
+  using V = Vec<T>;
+  constexpr int E = V::E;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
   const int64_t r = blockIdx.x / parts;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-  Row<T> row;
-  row.x = static_cast<const T*>(a.logits) + r * a.row_stride;
-  row.vocab = a.vocab;
-  row.shift = int((reinterpret_cast<uintptr_t>(row.x) & 15u) / sizeof(T));
-  const int64_t vectors = (a.vocab + row.shift + E - 1) / E;
-  const int64_t per = (vectors + parts - 1) / parts;
-  const int64_t v0 = part * per, v1 = v0 + per < vectors ? v0 + per : vectors;
+  const Row<T> row(static_cast<const T*>(a.logits) + r * a.row_stride, int(a.vocab));
+  const int per = (row.vectors + parts - 1) / parts;
+  const int v0 = min(row.vectors, part * per), v1 = min(row.vectors, v0 + per);
+  const bool edge = part == 0 && tid < row.edges;  // this thread also has an element at the row's ends
+  const float edge_x = edge ? to_f(row.x[row.edge(tid)]) : -INFINITY;
   if (tid == 0) sh.n_cand = 0, sh.n_elig = 0;
 
-  // ---- one pass: sums and each thread's greatest value
+  // ---- one pass: sums, and each thread's greatest value with the elements it was found among
   Sums st = {-INFINITY, 0.f, 0.f};
   float best = -INFINITY;
-  int64_t best_vec = v0 + tid;
-  for (int64_t j = v0 + tid; j < v1; j += kThreads * kBatch) {
-    uint4 v[kBatch];
-    float top[kBatch];
+  int best_first = 0, best_last = -1;
+  auto raise = [&](float to) {  // the running maximum
+    const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, to), f = st.m == -INFINITY ? 0.f : ex2(d);
+    st.u = f * (st.u + st.s * d);
+    st.s *= f;
+    st.m = to;
+  };
+  // log2 e times the maximum; 0 (every 2^t is 0 then) until there is one that the product holds
+  auto base = [&] { return st.m > V::kLow ? st.m * kLog2e : 0.f; };
+  auto batch = [&](const uint4* v, const int j, const int n) {
+    typename V::Top top[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int64_t jb = j + b * kThreads;
-      if (jb < v1) v[b] = row.load(jb);
-      else {
-        const T none = from_f<T>(-INFINITY);
-        T t[E];
+    for (int b = 0; b < kBatch; ++b) top[b] = V::top(v[b]);
+    typename V::Top all = top[0];
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] = none;
-        memcpy(&v[b], t, 16);
+    for (int b = 1; b < kBatch; ++b) all = V::greater(all, top[b]);
+    const float most = V::of_top(all);
+    if (most > st.m) raise(most);
+    if (most > best || best_last < 0) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const float x = V::of_top(top[b]);
+        if (b < n && (x > best || best_last < 0)) {
+          best = x == x ? x : -INFINITY;  // all NaN
+          best_first = row.first_of(j + b * kThreads);
+          best_last = best_first + E - 1;
+        }
       }
     }
-    float most = -INFINITY;
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      top[b] = Vec<T>::greatest(v[b]);
-      most = fmaxf(most, top[b]);
-      if (top[b] > best) {
-        best = top[b];
-        best_vec = j + b * kThreads;
-      }
-    }
-    if (most > st.m) {
-      const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, most), f = st.m == -INFINITY ? 0.f : ex2(d);
-      st.u = f * (st.u + st.s * d);
-      st.s *= f;
-      st.m = most;
-    }
-    const float base = st.m == -INFINITY ? 0.f : st.m;
+    const float m2 = base();
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       float x[E];
-      Vec<T>::to_floats(v[b], x);
+      V::clipped(v[b], x);
       float s = 0.f, u = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float t = (x[e] - base) * kLog2e;
-        const float p = ex2(t);
+        const float t = fmaf(x[e], kLog2e, -m2), p = ex2(t);
         s += p;
-        u = fmaf(p, fmaxf(t, -1e30f), u);  // 0 · -inf counts as 0
+        u = fmaf(p, t, u);
       }
       st.s += s;
       st.u += u;
     }
-  }
+  };
+  int j = v0 + tid;
+  for (; j + (kBatch - 1) * kThreads < v1; j += kBatch * kThreads) {
+    uint4 v[kBatch];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    Sums other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.u = __shfl_xor_sync(0xffffffffu, st.u, o);
-    st = join(st, other);
+    for (int b = 0; b < kBatch; ++b) v[b] = row.load(j + b * kThreads);
+    batch(v, j, kBatch);
   }
-  if (lane == 0) sh.sums[w] = st;
+  if (j < v1) {
+    uint4 v[kBatch];
+    const T none = from_f<T>(-INFINITY);
+    uint32_t word;
+    if constexpr (sizeof(T) == 4) word = __float_as_uint(-INFINITY);
+    else word = uint32_t(*reinterpret_cast<const unsigned short*>(&none)) * 0x10001u;
+    const int n = (v1 - j + kThreads - 1) / kThreads;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) v[b] = b < n ? row.load(j + b * kThreads) : make_uint4(word, word, word, word);
+    batch(v, j, n);
+  }
+  if (edge) {
+    if (edge_x > st.m) raise(edge_x);
+    const float x = edge_x < V::kClip ? V::kClip : edge_x;
+    const float t = fmaf(x, kLog2e, -base()), p = ex2(t);
+    st.s += p;
+    st.u = fmaf(p, t, st.u);
+    if (edge_x > best || best_last < 0) {
+      best = edge_x == edge_x ? edge_x : -INFINITY;
+      best_first = best_last = row.edge(tid);
+    }
+  }
+  auto block_join = [&] {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      Sums other;
+      other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+      other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+      other.u = __shfl_xor_sync(0xffffffffu, st.u, o);
+      st = join(st, other);
+    }
+    if (lane == 0) sh.sums[w] = st;
+    __syncthreads();
+  };
+  block_join();
+  float most = sh.sums[0].m;
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) most = fmaxf(most, sh.sums[i].m);
+  if (!(most > V::kLow && most < V::kHigh)) {
+    // element by element, without raising -inf and with the difference first
+    __syncthreads();
+    st = {most, 0.f, 0.f};
+    auto one = [&](float x) {
+      const float t = (x - (most == -INFINITY ? 0.f : most)) * kLog2e, p = ex2(t);
+      st.s += p;
+      st.u = fmaf(p, fmaxf(t, -1e30f), st.u);
+    };
+    for (int i = v0 + tid; i < v1; i += kThreads) {
+      float x[E];
+      V::to_floats(row.load(i), x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) one(x[e]);
+    }
+    if (edge) one(edge_x);
+    block_join();
+  }
 
   // ---- the k best of this CTA's part
   const int k = a.top;
   if (k) {
-    const bool has = v0 + tid < v1;
-    const int64_t i0 = best_vec * E - row.shift;
-    const uint32_t first = uint32_t(i0 < 0 ? 0 : i0), last = uint32_t(i0 + E - 1 < a.vocab ? i0 + E - 1 : a.vocab - 1);
-    Key mine = warp_sort(has ? key_of(best, last) : 0ull);
+    const bool has = best_last >= 0;
+    Key mine = warp_sort(has ? key_of(best, best_last) : 0ull);
     for (int n = kWarps; n > 1; n >>= 1) {
       if (w < n) sh.lists[w][lane] = mine;
       __syncthreads();
@@ -252,23 +324,22 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
     if (tid == k - 1) sh.tau = mine;  // 0 when fewer than k threads have elements: all are candidates
     __syncthreads();
     const Key tau = sh.tau;
-    if (has && key_of(best, first) >= tau) sh.elig[atomicAdd(&sh.n_elig, 1)] = tid;
+    if (has && key_of(best, best_first) >= tau) sh.elig[atomicAdd(&sh.n_elig, 1)] = tid;
     __syncthreads();
     const int n_elig = sh.n_elig;
+    auto offer = [&](Key key) {
+      if (key < tau) return;
+      const int at = atomicAdd(&sh.n_cand, 1);
+      if (at < kCandidates) sh.cand[at] = key;
+    };
     for (int q = w; q < n_elig; q += kWarps)
-      for (int64_t j = v0 + sh.elig[q] + int64_t(lane) * kThreads; j < v1; j += 32 * kThreads) {
+      for (int i = v0 + sh.elig[q] + lane * kThreads; i < v1; i += 32 * kThreads) {
         float x[E];
-        Vec<T>::to_floats(row.load(j), x);
+        V::to_floats(row.load(i), x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int64_t i = j * E - row.shift + e;
-          const Key key = key_of(x[e], uint32_t(i));
-          if (i >= 0 && i < a.vocab && key >= tau) {
-            const int at = atomicAdd(&sh.n_cand, 1);
-            if (at < kCandidates) sh.cand[at] = key;
-          }
-        }
+        for (int e = 0; e < E; ++e) offer(key_of(x[e], row.first_of(i) + e));
       }
+    if (edge) offer(key_of(edge_x, row.edge(tid)));
     __syncthreads();
     const int n = sh.n_cand;
     if (n <= kCandidates) {
@@ -288,16 +359,19 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
       for (int i = 0; i < 32; ++i) {
         Key top = 0ull;
         if (i < k)
-          for (int64_t j = v0 + tid; j < v1; j += kThreads) {
+          for (int v = v0 + tid; v < v1; v += kThreads) {
             float x[E];
-            Vec<T>::to_floats(row.load(j), x);
+            V::to_floats(row.load(v), x);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-              const int64_t at = j * E - row.shift + e;
-              const Key key = key_of(x[e], uint32_t(at));
-              if (at >= 0 && at < a.vocab && key < prev) top = max_key(top, key);
+              const Key key = key_of(x[e], row.first_of(v) + e);
+              if (key < prev) top = max_key(top, key);
             }
           }
+        if (i < k && edge) {
+          const Key key = key_of(edge_x, row.edge(tid));
+          if (key < prev) top = max_key(top, key);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = max_key(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) sh.lists[w][0] = top;
@@ -309,7 +383,6 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
       }
     }
   }
-  __syncthreads();
   if (tid == 0) {
     Sums all = sh.sums[0];
     for (int i = 1; i < kWarps; ++i) all = join(all, sh.sums[i]);
