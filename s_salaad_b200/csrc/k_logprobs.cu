@@ -15,12 +15,14 @@
 // lowest or greatest value) the part is summed again element by element.
 //
 // The k best need no second pass over the row: each thread also keeps its
-// greatest value and the vector that held it.  The k-th greatest of these
-// (a lower bound of the k-th greatest element) leaves about k threads that
-// can hold a better element; only their vectors are read again (from L2).
+// greatest value and the vector that held it, and (in shared memory) the
+// greatest value of each of up to 16 groups of its vectors.  The k-th greatest
+// of the threads' values is a lower bound of the k-th greatest element, which
+// leaves about k groups that can hold a better one; only they are read again,
+// all at once, and their elements from the bound on are ranked by counting.  (Reading the whole of the k threads' vectors again cost 14 us
+// of the 41 us that a row of 151936 took: they have left L2 by then.)
 // Elements are ordered by value, then by lower index, as unique 64-bit keys.
 #include <cooperative_groups.h>
-
 #include <type_traits>
 
 #include "internal.hpp"
@@ -33,10 +35,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;       // vectors in flight per thread
 constexpr int kCandidates = 512;
+constexpr int kGroups = 16;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -126,7 +129,14 @@ template <typename T, typename P> struct Vec16 {
   __device__ static P as(uint32_t w) { return *reinterpret_cast<P*>(&w); }
   __device__ static void unpack(const P* p, float* f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[2 * i] = to_f(p[i].x), f[2 * i + 1] = to_f(p[i].y);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of an fp32
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p + i);
+        f[2 * i] = __uint_as_float(w << 16), f[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+      } else {
+        f[2 * i] = to_f(p[i].x), f[2 * i + 1] = to_f(p[i].y);
+      }
+    }
   }
   __device__ static void to_floats(const uint4& v, float* f) {
     const P p[4] = {as(v.x), as(v.y), as(v.z), as(v.w)};
@@ -178,19 +188,20 @@ struct Shared {
   Key best[32];       // this CTA's list, greatest first
   Sums mine;
   Key tau, next;
-  int n_cand, n_elig, valid;
-  int elig[kThreads];
+  int n_cand, n_elig;
+  float group[kGroups][kThreads];               // greatest value of each thread's groups of batches
+  unsigned short elig[kGroups * kThreads];      // groups to read again
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs a) {
   using V = Vec<T>;
   constexpr int E = V::E;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
-  const int64_t r = blockIdx.x / parts;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
+  const int64_t r = blockIdx.x / parts;
   const Row<T> row(static_cast<const T*>(a.logits) + r * a.row_stride, int(a.vocab));
   const int per = (row.vectors + parts - 1) / parts;
   const int v0 = min(row.vectors, part * per), v1 = min(row.vectors, v0 + per);
@@ -201,7 +212,11 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
   // ---- one pass: sums, and each thread's greatest value with the elements it was found among
   Sums st = {-INFINITY, 0.f, 0.f};
   float best = -INFINITY;
-  int best_first = 0, best_last = -1;
+  int best_last = -1;  // index of the last element of the vector that held it
+  const int batches = (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch);
+  const int group_size = (batches + kGroups - 1) / kGroups;  // batches
+  int groups = 0, in_count = 0;
+  float in_group = -INFINITY;
   auto raise = [&](float to) {  // the running maximum
     const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, to), f = st.m == -INFINITY ? 0.f : ex2(d);
     st.u = f * (st.u + st.s * d);
@@ -219,14 +234,21 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
     for (int b = 1; b < kBatch; ++b) all = V::greater(all, top[b]);
     const float most = V::of_top(all);
     if (most > st.m) raise(most);
+    if (a.top) {
+      in_group = fmaxf(in_group, most);
+      if (++in_count == group_size) {
+        sh.group[groups++][tid] = in_group;
+        in_count = 0;
+        in_group = -INFINITY;
+      }
+    }
     if (most > best || best_last < 0) {
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const float x = V::of_top(top[b]);
         if (b < n && (x > best || best_last < 0)) {
           best = x == x ? x : -INFINITY;  // all NaN
-          best_first = row.first_of(j + b * kThreads);
-          best_last = best_first + E - 1;
+          best_last = row.first_of(j + b * kThreads) + E - 1;
         }
       }
     }
@@ -247,11 +269,24 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
     }
   };
   int j = v0 + tid;
-  for (; j + (kBatch - 1) * kThreads < v1; j += kBatch * kThreads) {
-    uint4 v[kBatch];
+  constexpr int kSpan = kBatch * kThreads;
+  auto whole = [&](int at) { return at + kSpan - kThreads < v1; };
+  auto fetch = [&](uint4* v, int at) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = row.load(j + b * kThreads);
+    for (int b = 0; b < kBatch; ++b) v[b] = row.load(at + b * kThreads);
+  };
+  // the next batch is under way while one is summed
+  if (whole(j)) {
+    uint4 v[kBatch], next[kBatch];
+    fetch(v, j);
+    for (; whole(j + kSpan); j += kSpan) {
+      fetch(next, j + kSpan);
+      batch(v, j, kBatch);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) v[b] = next[b];
+    }
     batch(v, j, kBatch);
+    j += kSpan;
   }
   if (j < v1) {
     uint4 v[kBatch];
@@ -272,18 +307,27 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
     st.u = fmaf(p, t, st.u);
     if (edge_x > best || best_last < 0) {
       best = edge_x == edge_x ? edge_x : -INFINITY;
-      best_first = best_last = row.edge(tid);
+      best_last = row.edge(tid);
     }
   }
-  auto block_join = [&] {
+  // the triples of a warp (or of its first lanes) as one, in every lane
+  auto warp_join = [&](Sums x) {
+    float top = x.m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float d = x.m == -INFINITY ? 0.f : log2_gap(x.m, top), f = x.m == -INFINITY ? 0.f : ex2(d);
+    x.u = f * (x.u + x.s * d);
+    x.s *= f;
+    x.m = top;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-      Sums other;
-      other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-      other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-      other.u = __shfl_xor_sync(0xffffffffu, st.u, o);
-      st = join(st, other);
+      x.s += __shfl_xor_sync(0xffffffffu, x.s, o);
+      x.u += __shfl_xor_sync(0xffffffffu, x.u, o);
     }
+    return x;
+  };
+  auto block_join = [&] {
+    st = warp_join(st);
     if (lane == 0) sh.sums[w] = st;
     __syncthreads();
   };
@@ -316,42 +360,46 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
     const bool has = best_last >= 0;
     Key mine = warp_sort(has ? key_of(best, best_last) : 0ull);
     for (int n = kWarps; n > 1; n >>= 1) {
-      if (w < n) sh.lists[w][lane] = mine;
+      if (w >= n / 2 && w < n) sh.lists[w][lane] = mine;
       __syncthreads();
       if (w < n / 2) mine = warp_merge(mine, sh.lists[w + n / 2][31 - lane]);
-      __syncthreads();
     }
     if (tid == k - 1) sh.tau = mine;  // 0 when fewer than k threads have elements: all are candidates
     __syncthreads();
     const Key tau = sh.tau;
-    if (has && key_of(best, best_first) >= tau) sh.elig[atomicAdd(&sh.n_elig, 1)] = tid;
+    const float tau_x = tau ? value_of(tau) : -INFINITY;
+    if (in_count) sh.group[groups++][tid] = in_group;
+    for (int g = 0; g < groups; ++g)
+      if (sh.group[g][tid] >= tau_x) sh.elig[atomicAdd(&sh.n_elig, 1)] = static_cast<unsigned short>(g * kThreads + tid);
     __syncthreads();
-    const int n_elig = sh.n_elig;
     auto offer = [&](Key key) {
       if (key < tau) return;
       const int at = atomicAdd(&sh.n_cand, 1);
       if (at < kCandidates) sh.cand[at] = key;
     };
-    for (int q = w; q < n_elig; q += kWarps)
-      for (int i = v0 + sh.elig[q] + lane * kThreads; i < v1; i += 32 * kThreads) {
-        float x[E];
-        V::to_floats(row.load(i), x);
+    const int sub = group_size * kBatch;  // vectors of a group
+    for (int q = tid; q < sh.n_elig * sub; q += kThreads) {
+      const int e = sh.elig[q / sub];
+      const int i = v0 + ((e / kThreads) * sub + q % sub) * kThreads + e % kThreads;
+      if (i >= v1) continue;
+      const uint4 v = row.load(i);
+      if (V::of_top(V::top(v)) < tau_x) continue;  // all NaN goes on
+      float x[E];
+      V::to_floats(v, x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) offer(key_of(x[e], row.first_of(i) + e));
-      }
+      for (int e2 = 0; e2 < E; ++e2) offer(key_of(x[e2], row.first_of(i) + e2));
+    }
     if (edge) offer(key_of(edge_x, row.edge(tid)));
     __syncthreads();
     const int n = sh.n_cand;
     if (n <= kCandidates) {
-      if (w == 0) {
-        Key list = 0ull;
-        for (int c = 0; c < n; c += 32) {
-          const Key chunk = warp_sort(c + lane < n ? sh.cand[c + lane] : 0ull);
-          const Key rev = __shfl_sync(0xffffffffu, chunk, 31 - lane);
-          list = warp_merge(list, rev);
-        }
-        sh.best[lane] = list;
+      for (int c = tid; c < n; c += kThreads) {
+        const Key mine = sh.cand[c];
+        int rank = 0;
+        for (int q = 0; q < n; ++q) rank += sh.cand[q] > mine;
+        if (rank < 32) sh.best[rank] = mine;
       }
+      if (tid >= n && tid < 32) sh.best[tid] = 0ull;
     } else {
       // more candidates than the buffer holds (long runs of nearly equal
       // values in a few threads): one element per round, the greatest below the last
@@ -383,10 +431,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a)
       }
     }
   }
-  if (tid == 0) {
-    Sums all = sh.sums[0];
-    for (int i = 1; i < kWarps; ++i) all = join(all, sh.sums[i]);
-    sh.mine = all;
+  if (w == 0) {
+    const Sums all = warp_join(lane < kWarps ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f});
+    if (lane == 0) sh.mine = all;
   }
   if (parts > 1) cluster.sync();
   else __syncthreads();
