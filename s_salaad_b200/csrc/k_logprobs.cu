@@ -16,9 +16,9 @@
 //
 // The k best need no second pass over the row: each thread also keeps its
 // greatest value and the vector that held it, and (in shared memory) the
-// greatest value of each of up to 16 groups of its vectors.  The k-th greatest
-// of the threads' values is a lower bound of the k-th greatest element, which
-// leaves about k groups that can hold a better one; only they are read again,
+// greatest value of each of up to 64 groups of its vectors.  The k-th greatest
+// of 64 sets of threads' values is a lower bound of the k-th greatest element, which
+// leaves about k groups (44 for k = 32) that can hold a better one; only they are read again,
 // all at once, and their elements from the bound on are ranked by counting.  (Reading the whole of the k threads' vectors again cost 14 us
 // of the 41 us that a row of 151936 took: they have left L2 by then.)
 // Elements are ordered by value, then by lower index, as unique 64-bit keys.
@@ -38,8 +38,12 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBatch = 4;       // vectors in flight per thread
+static_assert(kWarps == 4 && kBatch == 4, "the sets of threads, the groups of batches");
+constexpr int kPerSm = 8;       // CTAs per SM
 constexpr int kCandidates = 512;
-constexpr int kGroups = 16;
+constexpr int kEligible = 512;
+// Groups per thread; 8 CTAs per SM share what L1 leaves: 40 groups of fp32 were 15 % slower.
+template <typename T> constexpr int kGroups = sizeof(T) == 4 ? 20 : 64;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -47,6 +51,25 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 in one 64-bit register pair: one instruction for both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 struct Sums {
@@ -181,23 +204,23 @@ template <typename T> struct Row {
   __device__ int edge(int e) const { return e < head ? e : e + vectors * E; }
 };
 
-struct Shared {
+template <typename T> struct Shared {
   Sums sums[kWarps];
-  Key lists[kWarps][32];
+  Key lists[kWarps][32];  // sets of threads (and the warps' best in the slow search)
   Key cand[kCandidates];
   Key best[32];       // this CTA's list, greatest first
   Sums mine;
   Key tau, next;
   int n_cand, n_elig;
-  float group[kGroups][kThreads];               // greatest value of each thread's groups of batches
-  unsigned short elig[kGroups * kThreads];      // groups to read again
+  T group[kGroups<T>][kThreads];      // greatest value of each thread's groups of batches
+  unsigned short elig[kEligible];  // groups to read again
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const LogprobArgs a) {
   using V = Vec<T>;
   constexpr int E = V::E;
-  __shared__ Shared sh;
+  __shared__ Shared<T> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
@@ -213,9 +236,9 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs
   Sums st = {-INFINITY, 0.f, 0.f};
   float best = -INFINITY;
   int best_last = -1;  // index of the last element of the vector that held it
-  const int batches = (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch);
-  const int group_size = (batches + kGroups - 1) / kGroups;  // batches
-  int groups = 0, in_count = 0;
+  const int batches = max(1, (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch));
+  const int group_log = 32 - __clz((batches + kGroups<T> - 1) / kGroups<T> * 2 - 1) - 1;  // batches: a power of two
+  int n_batch = 0;
   float in_group = -INFINITY;
   auto raise = [&](float to) {  // the running maximum
     const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, to), f = st.m == -INFINITY ? 0.f : ex2(d);
@@ -235,12 +258,8 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs
     const float most = V::of_top(all);
     if (most > st.m) raise(most);
     if (a.top) {
-      in_group = fmaxf(in_group, most);
-      if (++in_count == group_size) {
-        sh.group[groups++][tid] = in_group;
-        in_count = 0;
-        in_group = -INFINITY;
-      }
+      in_group = (n_batch & ((1 << group_log) - 1)) ? fmaxf(in_group, most) : most;
+      sh.group[n_batch++ >> group_log][tid] = from_f<T>(in_group);  // exact
     }
     if (most > best || best_last < 0) {
 #pragma unroll
@@ -253,20 +272,27 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs
       }
     }
     const float m2 = base();
+    const Pair scale2 = pair(kLog2e, kLog2e), base2 = pair(-m2, -m2);
+    Pair s2 = 0, u2 = 0;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       float x[E];
       V::clipped(v[b], x);
-      float s = 0.f, u = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float t = fmaf(x[e], kLog2e, -m2), p = ex2(t);
-        s += p;
-        u = fmaf(p, t, u);
+      for (int e = 0; e < E; e += 2) {
+        const Pair t2 = fma2(pair(x[e], x[e + 1]), scale2, base2);
+        float t0, t1;
+        unpair(t2, t0, t1);
+        const Pair p2 = pair(ex2(t0), ex2(t1));
+        s2 = add2(s2, p2);
+        u2 = fma2(p2, t2, u2);
       }
-      st.s += s;
-      st.u += u;
     }
+    float s0, s1, u0, u1;
+    unpair(s2, s0, s1);
+    unpair(u2, u0, u1);
+    st.s += s0 + s1;
+    st.u += u0 + u1;
   };
   int j = v0 + tid;
   constexpr int kSpan = kBatch * kThreads;
@@ -279,14 +305,24 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs
   if (whole(j)) {
     uint4 v[kBatch], next[kBatch];
     fetch(v, j);
-    for (; whole(j + kSpan); j += kSpan) {
+    while (true) {
+      if (!whole(j + kSpan)) {
+        batch(v, j, kBatch);
+        j += kSpan;
+        break;
+      }
       fetch(next, j + kSpan);
       batch(v, j, kBatch);
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) v[b] = next[b];
+      j += kSpan;
+      if (!whole(j + kSpan)) {
+        batch(next, j, kBatch);
+        j += kSpan;
+        break;
+      }
+      fetch(v, j + kSpan);
+      batch(next, j, kBatch);
+      j += kSpan;
     }
-    batch(v, j, kBatch);
-    j += kSpan;
   }
   if (j < v1) {
     uint4 v[kBatch];
@@ -358,36 +394,62 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LogprobArgs
   const int k = a.top;
   if (k) {
     const bool has = best_last >= 0;
-    Key mine = warp_sort(has ? key_of(best, best_last) : 0ull);
-    for (int n = kWarps; n > 1; n >>= 1) {
-      if (w >= n / 2 && w < n) sh.lists[w][lane] = mine;
-      __syncthreads();
-      if (w < n / 2) mine = warp_merge(mine, sh.lists[w + n / 2][31 - lane]);
+    // 64 sets of two threads: sorted by two warps, merged by one
+    const Key own = has ? key_of(best, best_last) : 0ull;
+    if (w >= 2) sh.lists[w - 2][lane] = own;
+    __syncthreads();
+    if (w < 2) {
+      const Key mine = warp_sort(max_key(own, sh.lists[w][lane]));
+      if (w == 1) sh.lists[1][lane] = mine;
+      named_bar_sync(1, 64);
+      if (w == 0) {
+        const Key both = warp_merge(mine, sh.lists[1][31 - lane]);
+        if (lane == k - 1) sh.tau = both;  // 0 when fewer than k sets have elements: all are candidates
+      }
     }
-    if (tid == k - 1) sh.tau = mine;  // 0 when fewer than k threads have elements: all are candidates
     __syncthreads();
     const Key tau = sh.tau;
     const float tau_x = tau ? value_of(tau) : -INFINITY;
-    if (in_count) sh.group[groups++][tid] = in_group;
+    const int groups = (n_batch + (1 << group_log) - 1) >> group_log;
     for (int g = 0; g < groups; ++g)
-      if (sh.group[g][tid] >= tau_x) sh.elig[atomicAdd(&sh.n_elig, 1)] = static_cast<unsigned short>(g * kThreads + tid);
+      if (to_f(sh.group[g][tid]) >= tau_x) {
+        const int at = atomicAdd(&sh.n_elig, 1);
+        if (at < kEligible) sh.elig[at] = static_cast<unsigned short>(g * kThreads + tid);
+      }
     __syncthreads();
     auto offer = [&](Key key) {
       if (key < tau) return;
       const int at = atomicAdd(&sh.n_cand, 1);
       if (at < kCandidates) sh.cand[at] = key;
     };
-    const int sub = group_size * kBatch;  // vectors of a group
-    for (int q = tid; q < sh.n_elig * sub; q += kThreads) {
-      const int e = sh.elig[q / sub];
-      const int i = v0 + ((e / kThreads) * sub + q % sub) * kThreads + e % kThreads;
-      if (i >= v1) continue;
-      const uint4 v = row.load(i);
-      if (V::of_top(V::top(v)) < tau_x) continue;  // all NaN goes on
-      float x[E];
-      V::to_floats(v, x);
+    // four reads in flight per thread: the latency of DRAM counts here
+    const int sub_log = group_log + 2;
+    const bool all = sh.n_elig > kEligible;  // many equal values: every vector
+    const int items = all ? v1 - v0 : sh.n_elig << sub_log;
+    for (int q0 = tid; q0 < items; q0 += 4 * kThreads) {
+      uint4 v[4];
+      int at[4];
 #pragma unroll
-      for (int e2 = 0; e2 < E; ++e2) offer(key_of(x[e2], row.first_of(i) + e2));
+      for (int i = 0; i < 4; ++i) {
+        const int q = q0 + i * kThreads;
+        at[i] = v1;
+        if (all) {
+          at[i] = v0 + q;
+        } else if (q < items) {
+          const int e = sh.elig[q >> sub_log];
+          at[i] = v0 + (((e / kThreads) << sub_log) + (q & ((1 << sub_log) - 1))) * kThreads + e % kThreads;
+        }
+        if (at[i] < v1) v[i] = row.load(at[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (at[i] >= v1 || V::of_top(V::top(v[i])) < tau_x) continue;  // all NaN goes on
+        float x[E];
+        V::to_floats(v[i], x);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (!(x[e] < tau_x)) offer(key_of(x[e], row.first_of(at[i]) + e));
+      }
     }
     if (edge) offer(key_of(edge_x, row.edge(tid)));
     __syncthreads();
