@@ -52,17 +52,22 @@ __device__ __forceinline__ int64_t kept_length(const PagesK& p, const int32_t* p
 }
 
 // Table rows become their parents' rows, entries behind the kept length -1.
-// Columns are independent, so a CTA reads its columns of every row before it
-// writes them: in place, one launch.  refs follow by integer atomics; each
-// CTA adds its change of the number of live pages.
+// Columns are independent, so a CTA reads its kCols columns of every row
+// before it writes them: in place, one launch.  refs follow by integer
+// atomics; each CTA adds its change of the number of live pages.  Bound by the
+// atomics' latency: few columns per CTA (32 took 54 us for 250 rows x 120
+// pages, 4 take 6).
+constexpr int kCols = 4;
 __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32_t* parents, const int32_t* n_new,
-                                                     int n_all, int cols) {
+                                                     int n_all) {
   extern __shared__ int32_t sm[];
-  int32_t* old = sm;                    // [rows][cols]
-  int32_t* keep = old + p.rows * cols;  // [rows] entries kept
-  int32_t* from = keep + p.rows;        // [rows]
+  int32_t* old = sm;                     // [rows][kCols]
+  int32_t* keep = old + p.rows * kCols;  // [rows] entries kept
+  int32_t* from = keep + p.rows;         // [rows]
   __shared__ int s_most, s_live;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, c0 = blockIdx.x * kCols;
+  pdl_wait_primary();
+  pdl_launch_dependents();
   if (tid == 0) s_most = 0, s_live = 0;
   __syncthreads();
   bool bad = false;
@@ -74,23 +79,25 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
     const int64_t len = p.lens[r];
     most = max(most, int(min(int64_t(p.max_pages), pages_of(max(len, int64_t(0)), p.page_size))));
   }
-  atomicMax(&s_most, most);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((tid & 31) == 0) atomicMax(&s_most, most);
   if (bad && blockIdx.x == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
   __syncthreads();
-  const int c0 = blockIdx.x * cols;
   // no row has an entry from here on: there is nothing to move or to drop
   if (c0 >= s_most) return;
-  for (int i = tid; i < p.rows * cols; i += blockDim.x) {
-    const int r = i / cols, c = c0 + i % cols;
-    old[i] = c < p.max_pages ? p.table[int64_t(r) * p.max_pages + c] : -1;
+#pragma unroll 4
+  for (int i = tid; i < p.rows * kCols; i += blockDim.x) {
+    const int c = c0 + i % kCols;
+    old[i] = c < p.max_pages ? p.table[int64_t(i / kCols) * p.max_pages + c] : -1;
   }
   __syncthreads();
   int live = 0;
-  for (int i = tid; i < p.rows * cols; i += blockDim.x) {
-    const int r = i / cols, j = i % cols, c = c0 + j;
+#pragma unroll 4
+  for (int i = tid; i < p.rows * kCols; i += blockDim.x) {
+    const int r = i / kCols, j = i % kCols, c = c0 + j;
     if (c >= p.max_pages) continue;
     const int was = old[i];
-    const int now = from[r] >= 0 && c < keep[r] ? old[from[r] * cols + j] : -1;
+    const int now = from[r] >= 0 && c < keep[r] ? old[from[r] * kCols + j] : -1;
     if (was == now) continue;
     p.table[int64_t(r) * p.max_pages + c] = now;
     if (was >= p.num_pages || now >= p.num_pages) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
@@ -98,48 +105,66 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
     if (now >= 0 && now < p.num_pages) live += atomicAdd(p.refs + now, 1) == 0;
     if (was >= 0 && was < p.num_pages) live -= atomicAdd(p.refs + was, -1) == 1;
   }
-  if (live) atomicAdd(&s_live, live);
+  live = __reduce_add_sync(0xffffffffu, live);
+  if ((tid & 31) == 0 && live) atomicAdd(&s_live, live);
   __syncthreads();
   if (tid == 0 && s_live) atomicAdd(p.head + kLive, s_live);
 }
 
 constexpr int kGrowThreads = 1024;
+constexpr int kPer = 8;  // pages of a thread in one step of a scan over refs
 
-// Exclusive scan over the block; *total: the sum.  Ends with a barrier.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t* total) {
+// Exclusive scan over the block; *total: the sum.  `sums`: 32 words of shared
+// memory that no other thread still reads.  Ends with a barrier.
+template <typename I> __device__ __forceinline__ I block_scan(I v, I* sums, I* total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int64_t incl = v;
+  I incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    const I up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
+  if (lane == 31) sums[w] = incl;
   __syncthreads();
-  if (lane == 31) warp_sums[w] = incl;
-  __syncthreads();
-  int64_t before = 0, all = 0;
-  for (int i = 0; i < kGrowThreads / 32; ++i) {
-    const int64_t x = warp_sums[i];
-    before += i < w ? x : 0;
-    all += x;
+  const I mine = sums[lane];
+  I all = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const I up = __shfl_up_sync(0xffffffffu, all, o);
+    if (lane >= o) all += up;
   }
-  *total = all;
+  *total = __shfl_sync(0xffffffffu, all, 31);
+  const I before = __shfl_sync(0xffffffffu, all - mine, w);
+  __syncthreads();
   return before + incl - v;
 }
 
+// Bit j: page i0 + j is free.
+__device__ __forceinline__ unsigned free_mask(const PagesK& p, int64_t i0) {
+  unsigned mask = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (i0 + j < p.num_pages && p.refs[i0 + j] == 0) mask |= 1u << j;
+  return mask;
+}
+
 // Growth of every row: one CTA.  Pages are given out lowest number first in
-// row order, a row's copy of a shared last page before its new pages.
+// row order, a row's copy of a shared last page before its new pages.  Bound
+// by the latency of its chain of reads (parents, lens, table, refs).
 __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, const int32_t* parents,
-                                                            const int32_t* n_new, int n_all) {
+                                                               const int32_t* n_new, int n_all) {
   extern __shared__ int32_t sm[];
   int32_t* low = sm;              // [rows] kept lengths
   int32_t* start = low + p.rows;  // [rows + 1] pages given to the rows before
   int32_t* copy = start + p.rows + 1;
-  __shared__ int64_t warp_sums[kGrowThreads / 32];
-  __shared__ int s_over, s_bad;
+  __shared__ int64_t sums64[32];
+  __shared__ int sums[32];
+  __shared__ int s_over;
   const int tid = threadIdx.x;
-  if (tid == 0) s_over = 0, s_bad = 0;
-  __syncthreads();
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const unsigned first_free = free_mask(p, int64_t(tid) * kPer);  // read early: most calls need no more
+  if (tid == 0) s_over = 0;
   const int64_t cap = int64_t(p.max_pages) * p.page_size;
   bool bad = false;
   auto grow_of = [&](int r) -> int64_t {
@@ -158,19 +183,22 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     }
     return p.refs[last] > 1 ? last : -1;
   };
+  bool any = false;
   for (int r = tid; r < p.rows; r += kGrowThreads) {
     const int last = shared_last(r);
     copy[r] = last;
-    if (last >= 0) p.growers[last] = 0, p.first[last] = INT_MAX;
+    if (last >= 0) p.growers[last] = 0, p.first[last] = INT_MAX, any = true;
     if (low[r] + grow_of(r) > cap) atomicAdd(&s_over, 1);
   }
-  __syncthreads();
-  for (int r = tid; r < p.rows; r += kGrowThreads)
-    if (copy[r] >= 0) {
-      atomicAdd(p.growers + copy[r], 1);
-      atomicMin(p.first + copy[r], r);
-    }
-  __syncthreads();
+  any = __syncthreads_or(any);
+  if (any) {
+    for (int r = tid; r < p.rows; r += kGrowThreads)
+      if (copy[r] >= 0) {
+        atomicAdd(p.growers + copy[r], 1);
+        atomicMin(p.first + copy[r], r);
+      }
+    __syncthreads();
+  }
   // when every sharer grows, the lowest row keeps the page
   const int chunk = (p.rows + kGrowThreads - 1) / kGrowThreads;
   const int r0 = min(p.rows, tid * chunk), r1 = min(p.rows, r0 + chunk);
@@ -179,12 +207,11 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     return pages_of(low[r] + grow_of(r), p.page_size) - pages_of(low[r], p.page_size) + (copy[r] >= 0 ? 1 : 0);
   };
   for (int r = r0; r < r1; ++r) {
-    if (copy[r] >= 0 && __ldcg(p.growers + copy[r]) == __ldcg(p.refs + copy[r]) && __ldcg(p.first + copy[r]) == r)
-      copy[r] = -1;
+    if (copy[r] >= 0 && __ldcg(p.growers + copy[r]) == p.refs[copy[r]] && __ldcg(p.first + copy[r]) == r) copy[r] = -1;
     mine += need_of(r);
   }
   int64_t total = 0;
-  int64_t at = block_scan(mine, warp_sums, &total);
+  int64_t at = block_scan(mine, sums64, &total);
   const int over = s_over;
   bool fits = over == 0 && total <= p.num_pages;
   if (fits)
@@ -192,20 +219,16 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
       start[r] = int(at);
       at += need_of(r);
     }
-  if (tid == 0) start[p.rows] = int(total);
+  if (tid == 0) start[p.rows] = fits ? int(total) : 0;
   // the lowest `total` free pages
   int64_t found = 0;
   if (total > 0) {
-    constexpr int kPer = 8;
     for (int64_t base = 0; base < p.num_pages && (found < total || !fits); base += kGrowThreads * kPer) {
       const int64_t i0 = base + tid * kPer;
-      unsigned mask = 0;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (i0 + j < p.num_pages && __ldcg(p.refs + i0 + j) == 0) mask |= 1u << j;
-      int64_t sum = 0;
-      int64_t k = found + block_scan(__popc(mask), warp_sums, &sum);
-      if (fits)
+      const unsigned mask = base ? free_mask(p, i0) : first_free;
+      int sum = 0;
+      int64_t k = found + block_scan(__popc(mask), sums, &sum);
+      if (fits && k < total)
         for (int j = 0; j < kPer; ++j)
           if (mask >> j & 1u) {
             if (k < total) p.list[k] = int32_t(i0 + j);
@@ -216,7 +239,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
   }
   fits = fits && found >= total;
   __syncthreads();
-  if (bad) s_bad = 1;
+  if (bad) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
   if (fits) {
     for (int k = tid; k < total; k += kGrowThreads) {
       int lo = 0, hi = p.rows - 1;  // the last row that starts at or before k and takes a page
@@ -232,9 +255,9 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
       p.refs[page] = 1;
     }
     // the copies, in row order
-    int64_t copies = 0, n_mine = 0;
+    int copies = 0, n_mine = 0;
     for (int r = r0; r < r1; ++r) n_mine += copy[r] >= 0;
-    int64_t c = block_scan(n_mine, warp_sums, &copies);
+    int c = any ? block_scan(n_mine, sums, &copies) : 0;
     for (int r = r0; r < r1; ++r)
       if (copy[r] >= 0) {
         p.src[c] = copy[r];
@@ -246,7 +269,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     if (tid == 0) {
       p.head[kShort] = 0;
       p.head[kOver] = 0;
-      p.head[kCopies] = int(copies);
+      p.head[kCopies] = copies;
       p.head[kLive] += int(total);
     }
   } else {
@@ -257,41 +280,49 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
       p.head[kCopies] = 0;
     }
   }
-  __syncthreads();
-  if (tid == 0 && s_bad) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
 }
 
 // Plan of a compaction: one CTA.  Live pages from the live count on go to the
 // free numbers below it, both ascending: no page is both read and written.
 __global__ void __launch_bounds__(kGrowThreads, 1) compact_plan_kernel(const PagesK p) {
-  __shared__ int64_t warp_sums[kGrowThreads / 32];
+  __shared__ unsigned long long sums[32];
+  __shared__ int s_live;
   const int tid = threadIdx.x;
-  constexpr int kPer = 8;
-  int64_t mine = 0, live = 0;
-  for (int64_t i = tid; i < p.num_pages; i += kGrowThreads) mine += p.refs[i] > 0;
-  block_scan(mine, warp_sums, &live);
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (tid == 0) s_live = 0;
+  __syncthreads();
+  const unsigned first_free = free_mask(p, int64_t(tid) * kPer);
+  int mine = 0;
+  for (int64_t i0 = int64_t(tid) * kPer; i0 < p.num_pages; i0 += kGrowThreads * kPer) {
+    const unsigned f = i0 == int64_t(tid) * kPer ? first_free : free_mask(p, i0);
+    mine += int(min(int64_t(kPer), p.num_pages - i0)) - __popc(f);
+  }
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if ((tid & 31) == 0) atomicAdd(&s_live, mine);
+  __syncthreads();
+  const int64_t live = s_live;
   int64_t holes = 0, movers = 0;
   for (int64_t base = 0; base < p.num_pages; base += kGrowThreads * kPer) {
     const int64_t i0 = base + tid * kPer;
-    unsigned hole = 0, mover = 0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (i0 + j < p.num_pages) {
-        const bool used = p.refs[i0 + j] > 0;
-        if (i0 + j < live && !used) hole |= 1u << j;
-        if (i0 + j >= live && used) mover |= 1u << j;
-        if (i0 + j >= live) p.first[i0 + j] = -1;
-      }
+    const unsigned f = base ? free_mask(p, i0) : first_free;
+    // bits of the pages below the live count, and of those that exist
+    const int64_t n_low = live - i0, n_in = p.num_pages - i0;
+    const unsigned low = n_low <= 0 ? 0u : n_low >= kPer ? 0xffu : (1u << n_low) - 1;
+    const unsigned in = n_in <= 0 ? 0u : n_in >= kPer ? 0xffu : (1u << n_in) - 1;
+    const unsigned hole = f & low, mover = ~f & ~low & in;
+    for (unsigned rest = ~low & in; rest; rest &= rest - 1) p.first[i0 + __ffs(rest) - 1] = -1;
     // both counts in one scan
-    int64_t sum = 0;
-    const int64_t at = block_scan(int64_t(__popc(hole)) << 32 | __popc(mover), warp_sums, &sum);
-    int64_t h = holes + (at >> 32), m = movers + (at & 0xffffffff);
+    unsigned long long sum = 0;
+    const unsigned long long at =
+        block_scan(static_cast<unsigned long long>(__popc(hole)) << 32 | __popc(mover), sums, &sum);
+    int64_t h = holes + int64_t(at >> 32), m = movers + int64_t(at & 0xffffffffu);
     for (int j = 0; j < kPer; ++j) {
       if (hole >> j & 1u) p.dst[h++] = int32_t(i0 + j);
       if (mover >> j & 1u) p.src[m++] = int32_t(i0 + j);
     }
-    holes += sum >> 32;
-    movers += sum & 0xffffffff;
+    holes += int64_t(sum >> 32);
+    movers += int64_t(sum & 0xffffffffu);
   }
   __syncthreads();
   for (int64_t i = tid; i < movers; i += kGrowThreads) {
@@ -449,6 +480,24 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a, int esi
   }
 }
 
+// A launch that may start while the kernel before it ends; every kernel here
+// waits for that one (griddepcontrol.wait) before it reads anything.
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+  return SLR_OK;
+}
+
 int sm_count(int* out) {
   int dev = 0;
   SLR_CHECK_CUDA(cudaGetDevice(&dev));
@@ -489,17 +538,7 @@ int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, cudaStream_t s)
   if (rc) return rc;
   const int64_t pieces = ceil_div(p.page_bytes, int64_t(kCopyThreads) * kCopyUnroll * 16);
   const int64_t items = std::max<int64_t>(1, pieces * c.planes * most_pairs);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>(items, int64_t(sms) * 8)));
-  cfg.blockDim = dim3(kCopyThreads);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, copy_kernel<16>, c));
-  return SLR_OK;
+  return launch_after(copy_kernel<16>, dim3(unsigned(std::min<int64_t>(items, int64_t(sms) * 8))), kCopyThreads, 0, s, c);
 }
 
 }  // namespace
@@ -511,17 +550,17 @@ size_t kv_pages_workspace_size(int rows, int num_pages) {
 int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const int32_t* parents, cudaStream_t s) {
   const PagesK k = views(p);
   if (parents || n_new || n_all < 0) {
-    const int cols = p.rows <= 512 ? 32 : 8;
-    const size_t smem = (size_t(p.rows) * cols + 2 * size_t(p.rows)) * 4;
+    const size_t smem = size_t(p.rows) * (kCols + 2) * 4;
     // one limit for every size, so that concurrent callers set the same
-    constexpr int kMost = std::max(512 * 34, kAttendMaxRows * 10) * 4;
-    SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
-    select_kernel<<<unsigned(ceil_div(p.max_pages, cols)), 256, smem, s>>>(k, parents, n_new, n_all, cols);
-    SLR_CHECK_LAUNCH("kv select");
+    SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kAttendMaxRows * (kCols + 2) * 4));
+    const int rc = launch_after(select_kernel, dim3(unsigned(ceil_div(p.max_pages, kCols))), 256, smem, s, k, parents,
+                                n_new, n_all);
+    if (rc) return rc;
   }
   const size_t smem = (3 * size_t(p.rows) + 1) * 4;
-  grow_kernel<<<1, kGrowThreads, smem, s>>>(k, parents, n_new, n_all);
-  SLR_CHECK_LAUNCH("kv grow");
+  const int rc = launch_after(grow_kernel, dim3(1), kGrowThreads, smem, s, k, parents, n_new, n_all);
+  if (rc) return rc;
   CopyK c = {};
   c.src = k.src;
   c.dst = k.dst;
@@ -531,8 +570,8 @@ int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const
 
 int launch_kv_compact(const PagesArgs& p, cudaStream_t s) {
   const PagesK k = views(p);
-  compact_plan_kernel<<<1, kGrowThreads, 0, s>>>(k);
-  SLR_CHECK_LAUNCH("kv compact");
+  const int rc = launch_after(compact_plan_kernel, dim3(1), kGrowThreads, 0, s, k);
+  if (rc) return rc;
   CopyK c = {};
   c.src = k.src;
   c.dst = k.dst;
@@ -558,19 +597,10 @@ int launch_kv_append(const AppendArgs& a, cudaStream_t s) {
   const auto even = [&](int64_t stride) { return stride * e % 16 == 0; };
   const bool wide = aligned16(a.new_k) && aligned16(a.new_v) && even(a.k_row) && even(a.k_head) && even(a.v_row) &&
                     even(a.v_head) && a.dim * e % 16 == 0;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(ceil_div(a.tokens, 4)));
-  cfg.blockDim = dim3(128);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (wide) SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel<16>, a, e));
-  else if (e == 4) SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel<4>, a, e));
-  else SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, append_kernel<2>, a, e));
-  return SLR_OK;
+  const dim3 grid(unsigned(ceil_div(a.tokens, 4)));
+  if (wide) return launch_after(append_kernel<16>, grid, 128, 0, s, a, e);
+  if (e == 4) return launch_after(append_kernel<4>, grid, 128, 0, s, a, e);
+  return launch_after(append_kernel<2>, grid, 128, 0, s, a, e);
 }
 
 int read_and_clear_status_pages(unsigned* out) {
