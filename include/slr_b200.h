@@ -462,8 +462,9 @@ typedef struct slr_kv_cache {
   int32_t dtype;          /* slr_dtype */
 } slr_kv_cache;
 
-/* Device bytes of scratch for slr_kv_advance and slr_kv_compact / for
- * slr_kv_attend on the current device (0 on bad arguments).  256-byte aligned, not shared by calls that may overlap on
+/* Device bytes of scratch for slr_kv_advance and slr_kv_compact (0 on a bad
+ * descriptor) / for slr_kv_attend with these rows and heads on the current
+ * device (0 also when it needs none).  256-byte aligned, not shared by calls that may overlap on
  * the GPU, needs no initialisation and keeps nothing between calls. */
 SLR_API size_t slr_kv_pages_workspace_size(const slr_kv_cache* cache);
 SLR_API size_t slr_kv_attend_workspace_size(const slr_kv_cache* cache, int32_t rows, int32_t heads);

@@ -218,7 +218,7 @@ struct AttendArgs {
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
 };
-int attend_workspace_size(int dtype, int dim, int rows, int group, size_t* bytes);
+int attend_workspace_size(int dtype, int dim, int rows, int kv_heads, int group, int64_t longest, size_t* bytes);
 int launch_attend(const AttendArgs& a, cudaStream_t s);
 
 // New tokens' K and V into one layer's pages.

@@ -15,12 +15,19 @@
 // others leave (o, m, l) per part in the workspace and attend_join_kernel joins
 // them in part order, so results do not depend on timing.
 //
+// Few and short rows (the whole call is latency) take a cluster of 1 to 8 CTAs
+// per (row, head block) instead: its warps share the tiles and join through
+// shared memory, in one launch without workspace (one row of 100 tokens, 8
+// heads of 64: 3.2 us instead of 9.4).
+//
 // A warp streams its tiles through its own ring of cp.async stages, across the
 // ends of rows, and waits for no other warp; the page number of a stage is
 // fetched one stage ahead, the q of the next row (or head block) one row ahead.
 // 16-bit types: Q·Kᵀ and P·V on mma.sync with the query heads of the group as
 // the 16 rows of the MMA (the work is far below tcgen05's tile of 128 rows and
 // the tensor pipe is not the bound).  fp32: FFMA.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -32,6 +39,8 @@ namespace slr {
 __device__ unsigned g_status_attend;
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kMinTokens = 64;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -123,7 +132,7 @@ template <typename T, int DP_, int GT_> struct Cfg {
   static constexpr int kQ = kF32 && !kQRegs ? W * GT * DP * 4 : 0;
   static constexpr int kP = kF32 ? W * TT * GT * 4 : 0;
   static constexpr int kCnt = W * NS * 4;
-  static constexpr int kFixed = kRing + kQ + kP + kCnt + 64;
+  static constexpr int kFixed = kRing + kQ + kP + kCnt + 64 + GT * 8;
   static constexpr int kMinTiles = kMinTokens / TT;
 };
 
@@ -155,7 +164,9 @@ __device__ __forceinline__ void cursor_skip(Cursor& c, const int* lens, int rows
   cursor_next<TT>(c, lens, rows, hb);
 }
 
-template <typename T, int DP_, int GT_>
+// kSmall: a cluster = (row, head block), the tiles of the row dealt to its warps
+// in equal parts.
+template <typename T, int DP_, int GT_, bool kSmall>
 __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const AttendK a) {
   using C = Cfg<T, DP_, GT_>;
   constexpr int DP = C::DP, W = C::W, TT = C::TT, NS = C::NS, GT = C::GT;
@@ -166,6 +177,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   float* ps = reinterpret_cast<float*>(smem + C::kRing + C::kQ);
   int* cnt = reinterpret_cast<int*>(smem + C::kRing + C::kQ + C::kP);
   int* scratch = cnt + W * NS;                       // 16 words
+  float2* ml = reinterpret_cast<float2*>(scratch + 16);  // kSmall: [GT] maximum and sum of the CTA
   int* lens = reinterpret_cast<int*>(smem + C::kFixed);  // [rows]
 
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
@@ -175,6 +187,28 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
 
   // ---- this warp's part of the list of tiles
   const int64_t cap = int64_t(a.max_pages) * a.page_size;
+  Cursor c;
+  int64_t t_begin, t_end;
+  int worker = 0;
+  bool active = true;
+  if constexpr (kSmall) {
+    const int cs = int(cg::this_cluster().num_blocks()), rank = int(cg::this_cluster().block_rank());
+    c.b = int(blockIdx.x) / cs / hb;
+    c.h = int(blockIdx.x) / cs % hb;
+    int64_t n = a.lens[c.b];
+    if (n < 0 || n > cap) {
+      if (tid == 0 && rank == 0) atomicOr(&g_status_attend, SLR_BAD_INDEX_BIT);
+      n = n < 0 ? 0 : cap;
+    }
+    c.len = int(n);
+    c.ntiles = (c.len + TT - 1) / TT;
+    const int per = (c.ntiles + W * cs - 1) / (W * cs);
+    c.seg = 0;
+    c.tile = (rank * W + w) * per;
+    t_begin = c.tile;
+    t_end = min(c.ntiles, c.tile + per);
+    active = t_begin < t_end;
+  } else {
   const int chunk = (a.rows + kThreads - 1) / kThreads;
   const int r0 = tid * chunk, r1 = min(a.rows, r0 + chunk);
   int mine = 0;
@@ -222,11 +256,10 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     if (bad) atomicOr(&g_status_attend, SLR_BAD_INDEX_BIT);
   }
   __syncthreads();
-  const int worker = int(blockIdx.x) * W + w;
-  const int64_t t_begin = worker * per;
-  const int64_t t_end = t_begin + per < n_all ? t_begin + per : n_all;
+  worker = int(blockIdx.x) * W + w;
+  t_begin = worker * per;
+  t_end = t_begin + per < n_all ? t_begin + per : n_all;
   if (t_begin >= t_end) return;  // no barrier of the CTA from here on
-  Cursor c;
   c.b = scratch[4 + 2 * w];
   c.len = lens[c.b];
   c.ntiles = (c.len + TT - 1) / TT;
@@ -239,6 +272,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     if (c.tile >= c.ntiles) cursor_skip<TT>(c, lens, a.rows, hb);
   }
   if (c.place() >= t_end || c.b >= a.rows) return;
+  }
 
   // ---- the ring
   // Chunk `ch` of a token's row lies at ch ^ (row & 7): the eight rows of an
@@ -270,9 +304,9 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       if (g < GT && g0 + g < a.group && d < a.dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + g * a.q_head + d));
     }
   };
-  int page = fetch_page(f);
+  int page = active ? fetch_page(f) : 0;
   int load_slot = 0;
-  bool more = true;  // tiles left to load
+  bool more = active;  // tiles left to load
   auto load_stage = [&]() {
     if (more) {
       const int t0 = f.tile * TT;
@@ -317,11 +351,16 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
           }
         }
       }
-      cursor_next<TT>(f, lens, a.rows, hb);
-      more = f.b < a.rows && f.place() < t_end;
-      if (more) {
-        page = fetch_page(f);
-        if (f.tile == 0) prefetch_q();
+      if constexpr (kSmall) {
+        more = ++f.tile < t_end;
+        if (more) page = fetch_page(f);
+      } else {
+        cursor_next<TT>(f, lens, a.rows, hb);
+        more = f.b < a.rows && f.place() < t_end;
+        if (more) {
+          page = fetch_page(f);
+          if (f.tile == 0) prefetch_q();
+        }
       }
       load_slot = load_slot + 1 == NS ? 0 : load_slot + 1;
     }
@@ -340,7 +379,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
   constexpr int kOut = C::kF32 ? GT * (DP / 32) : NT * DP / 4;
   float m[kStat], l[kStat], o[kOut];
   constexpr int kQf = C::kF32 ? 1 : NT * DP / 8, kQr = C::kF32 && C::kQRegs ? GT * DP / 4 : 1;
-  constexpr bool kAhead = C::kF32 ? kQr > 1 && kQr <= 32 : kQf <= 32;  // the next q fits the registers too
+  constexpr bool kAhead = kSmall ? false : C::kF32 ? kQr > 1 && kQr <= 32 : kQf <= 32;  // the next q fits the registers too
   uint32_t qf[kQf], qf_next[kAhead && !C::kF32 ? kQf : 1];
   float qr[kQr], qr_next[kAhead && C::kF32 ? kQr : 1];
   auto reset = [&]() {
@@ -643,8 +682,109 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     }
   };
 
+  // kSmall: the warps' results joined through the place of their rings
+  auto finish_small = [&]() {
+    cp_async_wait<0>();
+#pragma unroll
+    for (int i = 0; i < kStat; ++i)
+#pragma unroll
+      for (int x = C::kF32 ? 1 : 4; x < (C::kF32 ? 8 : 32); x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+    __syncwarp();
+    constexpr int kO = DP + 4;  // floats of a head's row (bank offset 4)
+    static_assert(GT * kO * 4 + GT * 8 <= NS * C::kStage, "a warp's rows take its ring's place");
+    float* mine = reinterpret_cast<float*>(ring + w * NS * C::kStage);
+    if constexpr (C::kF32) {
+#pragma unroll
+      for (int g = 0; g < GT; ++g) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+          mine[g * kO + (DP == 64 ? lane * 2 + i : (i / 4) * 128 + lane * 4 + (i & 3))] = o[g * (DP / 32) + i];
+        if (lane == 0) mine[GT * kO + 2 * g] = m[g], mine[GT * kO + 2 * g + 1] = l[g];
+      }
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < DP / 4; ++i)
+          mine[(nt * 8 + (lane & 3) * 2 + (i & 1)) * kO + (i >> 2) * 16 + ((i >> 1) & 1) * 8 + (lane >> 2)] =
+              o[nt * (DP / 4) + i];
+      if (lane < 4)
+#pragma unroll
+        for (int i = 0; i < kStat; ++i) {
+          const int g = (i >> 1) * 8 + lane * 2 + (i & 1);
+          mine[GT * kO + 2 * g] = m[i], mine[GT * kO + 2 * g + 1] = l[i];
+        }
+    }
+    __syncthreads();
+    const int kvh = kv_head(c.h), g0 = (c.h - kvh * a.hblocks) * GT;
+    const int heads = min(GT, a.group - g0);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int cs = int(cluster.num_blocks());
+    float* part = reinterpret_cast<float*>(ring);
+    constexpr int kPart = NS * C::kStage / 4;
+    auto write = [&](int g, int d, float top, float sum, float y) {
+      const int head = kvh * a.group + g0 + g;
+      if (d < a.dim)
+        static_cast<T*>(a.out)[int64_t(c.b) * a.o_row + int64_t(head) * a.o_head + d] =
+            from_f<T>(sum == 0.f ? 0.f : y / sum);
+      if (d == 0 && a.lse)
+        a.lse[int64_t(c.b) * a.kv_heads * a.group + head] =
+            sum == 0.f ? -INFINITY : kLn2 * ((top == -INFINITY ? 0.f : top) + log2f(sum));
+    };
+    // a part without a finite score has sum 0, or NaN if a score was NaN
+    auto weight = [](float m, float l, float top) { return m == -INFINITY ? (l != l ? l : 0.f) : ex2(m - top); };
+    for (int i = tid; i < heads * DP; i += kThreads) {
+      const int g = i / DP, d = i % DP;
+      float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) top = fmaxf(top, part[j * kPart + GT * kO + 2 * g]);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float pl = part[j * kPart + GT * kO + 2 * g + 1];
+        const float fac = weight(part[j * kPart + GT * kO + 2 * g], pl, top);
+        sum = fmaf(pl, fac, sum);
+        y = fmaf(part[j * kPart + g * kO + d], fac, y);
+      }
+      if (cs == 1) {
+        write(g, d, top, sum, y);
+      } else {
+        part[g * kO + d] = y;  // read by this thread alone
+        if (d == 0) ml[g] = make_float2(top, sum);
+      }
+    }
+    if (cs == 1) return;
+    cluster.sync();
+    for (int i = int(cluster.block_rank()) * kThreads + tid; i < heads * DP; i += cs * kThreads) {
+      const int g = i / DP, d = i % DP;
+      float top = -INFINITY, sum = 0.f, y = 0.f;
+      for (int j = 0; j < cs; ++j) top = fmaxf(top, cluster.map_shared_rank(ml, j)[g].x);
+      for (int j = 0; j < cs; ++j) {
+        const float2 x = cluster.map_shared_rank(ml, j)[g];
+        const float fac = weight(x.x, x.y, top);
+        sum = fmaf(x.y, fac, sum);
+        y = fmaf(cluster.map_shared_rank(part, j)[g * kO + d], fac, y);
+      }
+      write(g, d, top, sum, y);
+    }
+    cluster.sync();  // the parts stay until they have been read
+  };
+
   reset();
-  load_q(c, qf, qr);
+  if (active) load_q(c, qf, qr);
+  if constexpr (kSmall) {
+    int slot = 0;
+    for (int64_t t = t_begin; t < t_end; ++t) {
+      load_stage();
+      cp_async_wait<NS - 1>();
+      __syncwarp();
+      const int valid = cnt_w[slot];
+      if (valid > 0) step(ring_w + slot * C::kStage, valid);
+      __syncwarp();  // the slot may be refilled
+      slot = slot + 1 == NS ? 0 : slot + 1;
+    }
+    finish_small();
+    return;
+  }
   load_next_q();
   int slot = 0;
   while (true) {
@@ -763,9 +903,11 @@ struct Inst {
     int n = dev < kDevices ? known[cls][dev].load(std::memory_order_acquire) : 0;
     if (n == 0) {
       int occ = 0, sms = 0;
-      SLR_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, DP, GT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      SLR_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, DP, GT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           C::kFixed + kAttendMaxRows * 4));
-      SLR_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, attend_kernel<T, DP, GT>, C::W * 32, *smem));
+      SLR_CHECK_CUDA(cudaFuncSetAttribute(attend_kernel<T, DP, GT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          C::kFixed + kAttendMaxRows * 4));
+      SLR_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, attend_kernel<T, DP, GT, false>, C::W * 32, *smem));
       SLR_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
       if (occ < 1) return fail(SLR_ERR_UNSUPPORTED, "attend: the kernel does not fit this device");
       n = sms * occ;
@@ -807,28 +949,36 @@ struct Inst {
     const int64_t kw = C::kF32 ? 4 : 2;
     a.q_wide = a.q_row % kw == 0 && a.q_head % kw == 0 && reinterpret_cast<uintptr_t>(a.q) % (kw * sizeof(T)) == 0;
     a.o_pairs = a.o_row % 2 == 0 && a.o_head % 2 == 0 && reinterpret_cast<uintptr_t>(a.out) % 4 == 0;
-    // no more warps than shares of tiles that rows of the greatest length could have
-    const int64_t most = int64_t(a.rows) * a.kv_heads * a.hblocks *
-                         ceil_div(int64_t(a.max_pages) * a.page_size, int64_t(C::TT) * C::kMinTiles);
-    if (most < a.workers) a.workers = int(round_up(most, C::W));
+    const int64_t longest = int64_t(a.max_pages) * a.page_size;
+    const int small = small_cluster(x.rows, a.kv_heads * a.hblocks, longest, a.workers / C::W);
+    a.workers = useful(a.workers, x.rows, a.kv_heads * a.hblocks, longest);
     uint8_t* ws = static_cast<uint8_t*>(x.workspace);
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + size_t(2 * a.workers) * C::GT * DP * 4);
     a.prefix = reinterpret_cast<int32_t*>(ws + size_t(2 * a.workers) * C::GT * (DP * 4 + 8));
-    if (need(a.workers, a.rows) > x.workspace_bytes)
+    if (!small && need(a.workers, a.rows) > x.workspace_bytes)
       return fail(SLR_ERR_WORKSPACE,
                   "attend: workspace too small, need " + std::to_string(need(a.workers, a.rows)) + " bytes");
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(std::max(small, 1));
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.workers / C::W);
+    cfg.gridDim = dim3(small ? a.rows * a.kv_heads * a.hblocks * small : a.workers / C::W);
     cfg.blockDim = dim3(C::W * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<T, DP, GT>, a));
+    if (small) {
+      cfg.numAttrs = 2;
+      SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<T, DP, GT, true>, a));
+      return SLR_OK;
+    }
+    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<T, DP, GT, false>, a));
     // warps per head of the join: a fourth of the parts that an even split of
     // the longest possible rows gives each (they are read four at a time)
     int wph = 1;
@@ -841,14 +991,35 @@ struct Inst {
     return SLR_OK;
   }
 
+  // CTAs per (row, head block) when the call is small, else 0.  All CTAs run at
+  // once; the cluster grows until a row of the greatest length gives a warp 2
+  // tiles (a tile takes 0.3 to 0.4 us, a cluster 1.2 us more than one CTA).
+  // Where it cannot grow for want of SMs, up to 8 tiles are taken (256 CTAs, 512
+  // tokens, 32 heads of 128: 11 us, split 16; 1024 ragged tokens would wait for
+  // the longest).  Clusters of 8 take up to 16, 8192 tokens, since rows are
+  // mostly shorter than their table (one row, 8 key heads of 128: 100 tokens 5.6
+  // us, split 11.4; 4000 tokens 11.4, split 13.2; at 16000 it would be 29, split 18).
+  static int small_cluster(int rows, int hb, int64_t longest, int ctas) {
+    constexpr int64_t kTokens = 2 * C::W * C::TT;
+    int cs = 1;
+    while (cs < 8 && longest > kTokens * cs && int64_t(rows) * hb * cs * 2 <= ctas) cs *= 2;
+    return int64_t(rows) * hb * cs <= ctas && longest <= kTokens * cs * (cs == 8 ? 8 : 4) ? cs : 0;
+  }
+  // No more warps than shares of tiles that rows of the greatest length could have.
+  static int useful(int workers, int rows, int hb, int64_t longest) {
+    const int64_t most = int64_t(rows) * hb * ceil_div(longest, int64_t(C::TT) * C::kMinTiles);
+    return most < workers ? int(round_up(std::max<int64_t>(most, 1), C::W)) : workers;
+  }
   static size_t need(int workers, int rows) {
     return size_t(2 * workers) * C::GT * (DP * 4 + 8) + size_t(rows + 1) * 4;
   }
-  static int size(int rows, size_t* out) {
+  static int size(int rows, int kv_heads, int group, int64_t longest, size_t* out) {
     size_t smem = 0;
     int workers = 0;
     int rc = prepare(rows, &smem, &workers);
-    *out = rc ? 0 : need(workers, rows);
+    const int hb = kv_heads * int(ceil_div(group, GT));
+    const bool small = !rc && small_cluster(rows, hb, longest, workers / C::W);
+    *out = rc || small ? 0 : need(useful(workers, rows, hb, longest), rows);
     return rc;
   }
 };
@@ -878,8 +1049,9 @@ template <typename F> int by_shape(int dtype, int dim, int group, F&& f) {
 
 }  // namespace
 
-int attend_workspace_size(int dtype, int dim, int rows, int group, size_t* bytes) {
-  return by_shape(dtype, dim, group, [&](auto inst) { return decltype(inst)::size(rows, bytes); });
+int attend_workspace_size(int dtype, int dim, int rows, int kv_heads, int group, int64_t longest, size_t* bytes) {
+  return by_shape(dtype, dim, group,
+                  [&](auto inst) { return decltype(inst)::size(rows, kv_heads, group, longest, bytes); });
 }
 
 int launch_attend(const AttendArgs& a, cudaStream_t s) {

@@ -10,6 +10,7 @@
 // and page order, so the state never depends on timing; the only atomics are
 // integer sums and minima.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -498,10 +499,21 @@ int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cuda
   return SLR_OK;
 }
 
-int sm_count(int* out) {
+// The device's SMs; on the first call for a device also its kernels' limits
+// (the same for every caller and size).
+int prepare_device(int* sms) {
+  constexpr int kDevices = 32;
+  static std::atomic<int> known[kDevices];
   int dev = 0;
   SLR_CHECK_CUDA(cudaGetDevice(&dev));
-  SLR_CHECK_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+  int n = dev < kDevices ? known[dev].load(std::memory_order_acquire) : 0;
+  if (!n) {
+    SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kAttendMaxRows * (kCols + 2) * 4));
+    SLR_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < kDevices) known[dev].store(n, std::memory_order_release);
+  }
+  *sms = n;
   return SLR_OK;
 }
 
@@ -525,7 +537,7 @@ PagesK views(const PagesArgs& p) {
   return k;
 }
 
-int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, cudaStream_t s) {
+int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, int sms, cudaStream_t s) {
   c.k = p.k;
   c.v = p.v;
   c.layer_bytes = p.layer_bytes;
@@ -533,9 +545,6 @@ int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, cudaStream_t s)
   c.page_bytes = p.page_bytes;
   c.planes = 2 * p.layers;
   c.num_pages = p.num_pages;
-  int sms = 0;
-  int rc = sm_count(&sms);
-  if (rc) return rc;
   const int64_t pieces = ceil_div(p.page_bytes, int64_t(kCopyThreads) * kCopyUnroll * 16);
   const int64_t items = std::max<int64_t>(1, pieces * c.planes * most_pairs);
   return launch_after(copy_kernel<16>, dim3(unsigned(std::min<int64_t>(items, int64_t(sms) * 8))), kCopyThreads, 0, s, c);
@@ -549,28 +558,31 @@ size_t kv_pages_workspace_size(int rows, int num_pages) {
 
 int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const int32_t* parents, cudaStream_t s) {
   const PagesK k = views(p);
+  int sms = 0;
+  int rc = prepare_device(&sms);
+  if (rc) return rc;
   if (parents || n_new || n_all < 0) {
     const size_t smem = size_t(p.rows) * (kCols + 2) * 4;
-    // one limit for every size, so that concurrent callers set the same
-    SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        kAttendMaxRows * (kCols + 2) * 4));
-    const int rc = launch_after(select_kernel, dim3(unsigned(ceil_div(p.max_pages, kCols))), 256, smem, s, k, parents,
+    rc = launch_after(select_kernel, dim3(unsigned(ceil_div(p.max_pages, kCols))), 256, smem, s, k, parents,
                                 n_new, n_all);
     if (rc) return rc;
   }
   const size_t smem = (3 * size_t(p.rows) + 1) * 4;
-  const int rc = launch_after(grow_kernel, dim3(1), kGrowThreads, smem, s, k, parents, n_new, n_all);
+  rc = launch_after(grow_kernel, dim3(1), kGrowThreads, smem, s, k, parents, n_new, n_all);
   if (rc) return rc;
   CopyK c = {};
   c.src = k.src;
   c.dst = k.dst;
   c.count = k.head + kCopies;
-  return copy_launch(p, c, p.rows, s);
+  return copy_launch(p, c, p.rows, sms, s);
 }
 
 int launch_kv_compact(const PagesArgs& p, cudaStream_t s) {
   const PagesK k = views(p);
-  const int rc = launch_after(compact_plan_kernel, dim3(1), kGrowThreads, 0, s, k);
+  int sms = 0;
+  int rc = prepare_device(&sms);
+  if (rc) return rc;
+  rc = launch_after(compact_plan_kernel, dim3(1), kGrowThreads, 0, s, k);
   if (rc) return rc;
   CopyK c = {};
   c.src = k.src;
@@ -580,16 +592,19 @@ int launch_kv_compact(const PagesArgs& p, cudaStream_t s) {
   c.to = k.first;
   c.live = k.head + kLive;
   c.entries = int64_t(p.rows) * p.max_pages;
-  return copy_launch(p, c, std::max<int64_t>(p.num_pages / 2, ceil_div(c.entries, 1024)), s);
+  return copy_launch(p, c, std::max<int64_t>(p.num_pages / 2, ceil_div(c.entries, 1024)), sms, s);
 }
 
 int launch_kv_copy(const PagesArgs& p, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
+  int sms = 0;
+  const int rc = prepare_device(&sms);
+  if (rc) return rc;
   CopyK c = {};
   c.src = src;
   c.dst = dst;
   c.n = n;
   c.check = true;
-  return copy_launch(p, c, n, s);
+  return copy_launch(p, c, n, sms, s);
 }
 
 int launch_kv_append(const AppendArgs& a, cudaStream_t s) {

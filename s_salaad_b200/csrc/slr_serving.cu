@@ -93,7 +93,10 @@ size_t slr_kv_attend_workspace_size(const slr_kv_cache* cache, int32_t rows, int
     return 0;
   }
   size_t n = 0;
-  return attend_workspace_size(cache->dtype, cache->head_dim, rows, heads / cache->kv_heads, &n) ? 0 : n;
+  const int64_t longest = int64_t(cache->max_pages) * cache->page_size;
+  return attend_workspace_size(cache->dtype, cache->head_dim, rows, cache->kv_heads, heads / cache->kv_heads, longest, &n)
+             ? 0
+             : n;
 }
 
 int slr_kv_advance(const slr_kv_cache* cache, const int32_t* parents, const int32_t* n_new, int32_t n_all,
@@ -175,8 +178,7 @@ int slr_kv_attend(const slr_kv_cache* cache, int32_t layer, const void* q, int64
     return fail(SLR_ERR_UNSUPPORTED, "kv attend: max_rows * max_pages * page_size must be below 2^36");
   if (rows == 0) return SLR_OK;
   if (!q || !out) return fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: q or out is NULL");
-  rc = check_workspace(workspace, workspace_bytes, 1);
-  if (rc) return rc;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(SLR_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   AttendArgs a;
   a.k = layer_base(*cache, cache->k, layer);
   a.v = layer_base(*cache, cache->v, layer);

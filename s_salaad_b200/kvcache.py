@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DeviceGuard, _no_graph, _ptr, _require_cuda, _stream, slr_dtype
+from .ops import _DeviceGuard, _no_graph, _require_cuda, _stream, slr_dtype
 
 HEADER = _lib.SLR_KV_HEADER_WORDS
 
@@ -114,6 +114,7 @@ class PagedCache:
         if not self._pages_ws:
             raise ValueError(f"PagedCache: {_lib.last_error()}")
         self._attend_ws: dict = {}
+        self._index = device.index  # calls compare this number: cheaper than torch.device
 
     def _stride(self, i: int) -> int:
         """Stride of pool dimension i; of one of size 1, the packed one."""
@@ -129,11 +130,12 @@ class PagedCache:
 
     # ------------------------------------------------------ book-keeping --
     def _vector(self, name: str, t: torch.Tensor, n: int) -> torch.Tensor:
-        if t.dtype != torch.int32:
+        """int32 [n] on the cache's device, contiguous."""
+        if t.dtype is not torch.int32:
             raise TypeError(f"{name} must be int32, got {t.dtype}")
-        if t.device != self.device or tuple(t.shape) != (n,):
+        if t.get_device() != self._index or t.dim() != 1 or t.shape[0] != n:
             raise ValueError(f"{name} must be [{n}] on {self.device}")
-        return t.contiguous()
+        return t if t.is_contiguous() else t.contiguous()
 
     def advance(self, n_new: int | torch.Tensor = 1, parents: torch.Tensor | None = None) -> None:
         """The book-keeping of one step, for all rows at once.
@@ -162,9 +164,10 @@ class PagedCache:
             parents = self._vector("parents", parents, self.max_seqs)
         with _DeviceGuard(self.device):
             ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=self.device)
-            rc = self._lib.slr_kv_advance(self._ref, _ptr(parents), n_ptr, n_all, ws.data_ptr(), self._pages_ws,
-                                          _stream(self.device))
-        _lib.check(rc, "kv_advance")
+            rc = self._lib.slr_kv_advance(self._ref, None if parents is None else parents.data_ptr(), n_ptr, n_all,
+                                          ws.data_ptr(), self._pages_ws, _stream(self.device))
+        if rc:
+            _lib.check(rc, "kv_advance")
 
     def compact(self) -> None:
         """Moves the live pages to the lowest numbers (order kept among the
@@ -173,7 +176,8 @@ class PagedCache:
         with _DeviceGuard(self.device):
             ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=self.device)
             rc = self._lib.slr_kv_compact(self._ref, ws.data_ptr(), self._pages_ws, _stream(self.device))
-        _lib.check(rc, "kv_compact")
+        if rc:
+            _lib.check(rc, "kv_compact")
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Copies pages ``src[i]`` to ``dst[i]`` (int32) of every layer; the
@@ -204,15 +208,20 @@ class PagedCache:
                                f"{self.max_pages} pages")
 
     # ---------------------------------------------------------- per layer --
-    def _tokens(self, name: str, t: torch.Tensor) -> None:
-        if t.dtype != self.dtype:
+    def _tokens(self, name: str, t: torch.Tensor) -> tuple:
+        """(shape, strides) of [tokens, heads, head_dim] on the cache's device."""
+        if t.dtype is not self.dtype:
             raise TypeError(f"{name} must be {self.dtype}, got {t.dtype}")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name} must be on {self.device}, got {t.device}")
-        if t.dim() != 3 or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}], got {tuple(t.shape)}")
-        if t.stride(2) != 1:
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[2] != self.head_dim:
+            raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}], got {tuple(shape)}")
+        if stride[2] != 1:
             raise ValueError(f"{name} must have unit stride in the last dimension")
+        if t.requires_grad:
+            _no_graph(f"PagedCache ({name})", t)
+        return shape, stride
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_tokens: torch.Tensor | None = None) -> None:
         """Writes new tokens' keys and values [tokens, kv_heads, head_dim]
@@ -220,18 +229,19 @@ class PagedCache:
         its last positions.  ``cu_tokens`` (int32 [max_seqs + 1]): row b's
         tokens are ``[cu[b], cu[b + 1])``, further ones are padding.  Without
         it token i is row i's, and empty rows are skipped."""
-        self._tokens("k", k)
-        self._tokens("v", v)
-        if k.shape != v.shape or k.shape[1] != self.kv_heads:
+        shape, ks = self._tokens("k", k)
+        v_shape, vs = self._tokens("v", v)
+        if shape != v_shape or shape[1] != self.kv_heads:
             raise ValueError(f"k and v must be [tokens, {self.kv_heads}, {self.head_dim}]")
-        _no_graph("PagedCache.append", k, v)
+        cu = None
         if cu_tokens is not None:
             cu_tokens = self._vector("cu_tokens", cu_tokens, self.max_seqs + 1)
+            cu = cu_tokens.data_ptr()
         with _DeviceGuard(self.device):
-            rc = self._lib.slr_kv_append(self._ref, layer, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                         v.stride(0), v.stride(1), k.shape[0], _ptr(cu_tokens),
-                                         _stream(self.device))
-        _lib.check(rc, "kv_append")
+            rc = self._lib.slr_kv_append(self._ref, layer, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                         shape[0], cu, _stream(self.device))
+        if rc:
+            _lib.check(rc, "kv_append")
 
     def attend(self, layer: int, q: torch.Tensor, *, scale: float | None = None, out: torch.Tensor | None = None,
                return_lse: bool = False):
@@ -241,18 +251,18 @@ class PagedCache:
         row; ``scale`` defaults to ``head_dim ** -0.5``.  Empty rows give zeros.
         Returns ``out``, or ``(out, lse)`` with the float32 log-sum-exp
         [rows, heads] (-inf for empty rows)."""
-        self._tokens("q", q)
-        rows, heads = q.shape[0], q.shape[1]
+        shape, qs = self._tokens("q", q)
+        rows, heads, dim = shape
         if rows > self.max_seqs or heads == 0 or heads % self.kv_heads:
             raise ValueError(f"q must have at most {self.max_seqs} rows and a multiple of {self.kv_heads} heads, "
-                             f"got {tuple(q.shape)}")
-        _no_graph("PagedCache.attend", q)
+                             f"got {tuple(shape)}")
         if out is None:
-            out = torch.empty(rows, heads, self.head_dim, dtype=self.dtype, device=self.device)
+            out = torch.empty(rows, heads, dim, dtype=self.dtype, device=self.device)
+            os = (heads * dim, dim)
         else:
-            self._tokens("out", out)
-            if out.shape != q.shape:
-                raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+            out_shape, os = self._tokens("out", out)
+            if out_shape != shape:
+                raise ValueError(f"out must be {tuple(shape)}, got {tuple(out_shape)}")
         lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device) if return_lse else None
         with _DeviceGuard(self.device):
             need = self._attend_ws.get((rows, heads))
@@ -261,10 +271,11 @@ class PagedCache:
                 if len(self._attend_ws) > 256:
                     self._attend_ws.clear()
                 self._attend_ws[(rows, heads)] = need
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device).data_ptr() if need else None
             rc = self._lib.slr_kv_attend(
-                self._ref, layer, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-                out.stride(1), _ptr(lse), rows, heads, self.head_dim ** -0.5 if scale is None else scale,
-                ws.data_ptr(), need, _stream(self.device))
-        _lib.check(rc, "kv_attend")
+                self._ref, layer, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+                lse.data_ptr() if return_lse else None, rows, heads, dim ** -0.5 if scale is None else scale,
+                ws, need, _stream(self.device))
+        if rc:
+            _lib.check(rc, "kv_attend")
         return (out, lse) if return_lse else out

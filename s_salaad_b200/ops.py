@@ -690,34 +690,49 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     target from vocab on gives NaN and ``SLR_ERR_BAD_INDEX`` from
     ``slr_device_status`` (the call itself does not wait for the GPU).
     """
-    lib = _lib.load()
-    _require_cuda("logits", logits)
     dtype = slr_dtype(logits.dtype)
-    if logits.dim() < 1:
+    dev = logits.device
+    if dev.type != "cuda":
+        _require_cuda("logits", logits)
+    full = logits.shape
+    if not full:
         raise ValueError("logits must have at least one dimension")
-    vocab = logits.shape[-1]
+    vocab, shape = full[-1], full[:-1]
     if not 0 <= top <= min(_lib.SLR_MAX_TOP, vocab):
         raise ValueError(f"top must be in [0, min({_lib.SLR_MAX_TOP}, vocab)], got {top}")
     if targets is not None:
-        if targets.dtype != torch.int64:
+        if targets.dtype is not torch.int64:
             raise TypeError(f"targets must be int64, got {targets.dtype}")
-        if targets.device != logits.device or targets.shape != logits.shape[:-1]:
-            raise ValueError(f"targets must be {tuple(logits.shape[:-1])} on {logits.device}")
-        targets = targets.contiguous()
-    _no_graph("token_logprobs", logits)
-    shape, dev = logits.shape[:-1], logits.device
-    x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < vocab):
-        x = x.contiguous()
+        if targets.shape != shape or targets.get_device() != dev.index:
+            raise ValueError(f"targets must be {tuple(shape)} on {dev}")
+        if not targets.is_contiguous():
+            targets = targets.contiguous()
+    if logits.requires_grad:
+        _no_graph("token_logprobs", logits)
+    x = logits if len(full) == 2 else logits.reshape(-1, vocab)
     rows = x.shape[0]
-    lp = torch.empty(shape, dtype=torch.float32, device=dev) if targets is not None else None
-    ent = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
-    ids = torch.empty(*shape, top, dtype=torch.int64, device=dev) if top else None
-    val = torch.empty(*shape, top, dtype=torch.float32, device=dev) if top else None
+    stride, unit = x.stride()
+    if unit != 1 or (rows > 1 and stride < vocab):
+        x = x.contiguous()
+        stride = vocab
+    # (sizes as numbers: torch parses a tuple of them half as fast)
+    lp = None if targets is None else torch.empty(rows, dtype=torch.float32, device=dev)
+    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
+    ids = val = None
+    if top:
+        ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
+        val = torch.empty(rows, top, dtype=torch.float32, device=dev)
     with _DeviceGuard(dev):
-        rc = lib.slr_token_logprobs(x.data_ptr(), x.stride(0) if rows > 1 else vocab, rows, vocab, dtype,
-                                    _ptr(targets), _ptr(lp), _ptr(ent), top, _ptr(ids), _ptr(val), _stream(dev))
-    _lib.check(rc, "token_logprobs")
+        rc = _lib.load().slr_token_logprobs(
+            x.data_ptr(), stride if rows > 1 else vocab, rows, vocab, dtype,
+            None if lp is None else targets.data_ptr(), None if lp is None else lp.data_ptr(),
+            None if ent is None else ent.data_ptr(), top, None if ids is None else ids.data_ptr(),
+            None if val is None else val.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc, "token_logprobs")
+    if len(full) != 2:
+        lp, ent = (None if t is None else t.view(shape) for t in (lp, ent))
+        ids, val = (None if t is None else t.view(*shape, top) for t in (ids, val))
     return TokenLogprobs(lp, ent, ids, val)
 
 

@@ -88,6 +88,32 @@ def test_most_rows(cuda):
     assert not bool(got.any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 8), (128, 32, 8), (256, 20, 1), (40, 3, 3)])
+@pytest.mark.parametrize("width", [None, 30, 900, 5000])
+def test_few_short_rows(cuda, dtype, dim, heads, kv_heads, width):
+    """Short rows with a short table (one launch) and with a long one (split and joined)."""
+    lens = [3, 0, 17, 64, 130]
+    cache, k, v = filled_cache(lens, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype, width=width)
+    _check(cache, k, v, _q(5, heads, dim, dtype), None)
+
+
+def test_workspace_too_small_is_refused(cuda):
+    import ctypes
+
+    from s_salaad_b200 import _lib
+
+    cache, _, _ = filled_cache([20], kv_heads=1, dim=64, page=16, width=100000)
+    q, out = _q(1, 1, 64, BF16), torch.empty(1, 1, 64, dtype=BF16, device="cuda")
+    lib, ref = _lib.load(), ctypes.byref(cache.struct)
+    need = lib.slr_kv_attend_workspace_size(ref, 1, 1)
+    assert need > 0 and lib.slr_kv_attend_workspace_size(ref, 2, 1) == 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    for ptr, size in ((None, 0), (ws.data_ptr(), need - 1)):
+        rc = lib.slr_kv_attend(ref, 0, q.data_ptr(), 64, 64, out.data_ptr(), 64, 64, None, 1, 1, 1.0, ptr, size, None)
+        assert rc == _lib.SLR_ERR_WORKSPACE and "workspace" in _lib.last_error()
+
+
 def test_fewer_rows_than_the_cache_holds(cuda):
     lens = [40, 50, 60]
     cache, k, v = filled_cache(lens, kv_heads=2, dim=64, page=16)

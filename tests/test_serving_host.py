@@ -65,7 +65,7 @@ def test_bad_arguments():
                                       (0, 1, 8192, 1.0), (0, 1, 4, float("inf"))):
         assert lib.slr_kv_attend(ref, layer, 256, 1, 1, 256, 1, 1, None, rows, heads, scale, 256, need, None) == bad
     assert lib.slr_kv_attend(ref, 0, None, 1, 1, 256, 1, 1, None, 1, 4, 1.0, 256, need, None) == bad
-    assert lib.slr_kv_attend(ref, 0, 256, 1, 1, 256, 1, 1, None, 1, 4, 1.0, None, 0, None) == _lib.SLR_ERR_WORKSPACE
+    assert lib.slr_kv_attend(ref, 0, 256, 1, 1, 256, 1, 1, None, 1, 4, 1.0, 8, need, None) == _lib.SLR_ERR_WORKSPACE
     huge = ctypes.byref(_cache(max_rows=2048, max_pages=1 << 22))
     assert lib.slr_kv_attend(huge, 0, 256, 1, 1, 256, 1, 1, None, 1, 4, 1.0, 256, need,
                              None) == _lib.SLR_ERR_UNSUPPORTED
