@@ -33,11 +33,17 @@ def _next_token(logits: torch.Tensor) -> torch.Tensor:
 
 
 @torch.inference_mode()
-def generate(model, input_ids: torch.Tensor, max_new_tokens: int) -> torch.Tensor:
+def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, paged: bool = False) -> torch.Tensor:
     """Greedy decoding of ``max_new_tokens`` tokens after ``input_ids``
     [batch, prompt]; returns [batch, prompt + max_new_tokens].  One model
     forward per new token, as in the reference: the prompt (with the cache
-    filled), then each chosen token alone with the cache."""
+    filled), then each chosen token alone with the cache.  ``paged`` keeps the
+    keys and values in a :class:`~s_salaad_b200.kvcache.PagedCache` and attends
+    with its kernel, instead of the model's own growing cache."""
+    if paged:
+        from .paged import generate_paged
+
+        return generate_paged(model, input_ids, max_new_tokens)
     _check_request(model, input_ids, max_new_tokens)
     if max_new_tokens == 0:
         return input_ids

@@ -1,0 +1,183 @@
+"""Generation and scoring on the paged key-value cache.
+
+The reference decodes greedily and recomputes the prefix every step
+(``ssalaad/inference/generate.py:12-26``).  Here the keys and values of every
+sequence live in a :class:`~s_salaad_b200.kvcache.PagedCache`, the model's
+attention layers append to it and read it through an attention function
+registered with Hugging Face, and the tokens are chosen by
+:func:`~s_salaad_b200.ops.token_logprobs`; no step waits for the GPU.
+
+* :func:`generate_paged` — greedy decoding (``generate(..., paged=True)``);
+* :func:`beam_search` — the ``beams`` most probable continuations found by beam
+  search: hypotheses fork and end by page reference, only a shared last page is
+  copied;
+* :func:`score` — log probability of every token of given sequences.
+"""
+from __future__ import annotations
+
+import contextlib
+import threading
+
+import torch
+
+from ..kvcache import PagedCache
+from ..ops import TokenLogprobs, token_logprobs
+
+_ATTENTION = "slr_paged"
+_active = threading.local()  # .cache, .cu_tokens: set while a model runs on a cache
+
+
+def _paged_attention(module, query, key, value, attention_mask, scaling=None, **kwargs):
+    """Hugging Face attention function: query [rows, heads, T, head_dim], key
+    and value [rows, kv_heads, T, head_dim] of the T new tokens of each row."""
+    if kwargs.get("sliding_window") is not None:
+        raise ValueError("the paged cache has no sliding-window attention")
+    cache, layer = _active.cache, module.layer_idx
+    rows, heads, new, dim = query.shape
+    if new == 1:
+        cache.append(layer, key[:, :, 0], value[:, :, 0])
+        return cache.attend(layer, query[:, :, 0], scale=scaling)[:, None], None
+    # a prompt: attention among its own tokens, which start their rows
+    k, v = (t.transpose(1, 2).reshape(rows * new, -1, dim) for t in (key, value))
+    cache.append(layer, k, v, _active.cu_tokens)
+    out = torch.nn.functional.scaled_dot_product_attention(query, key, value, is_causal=True, scale=scaling,
+                                                           enable_gqa=heads != key.shape[1])
+    return out.transpose(1, 2), None
+
+
+@contextlib.contextmanager
+def _on_cache(model, cache: PagedCache):
+    """Within the block the model's attention layers use the cache."""
+    from transformers import AttentionInterface
+
+    AttentionInterface.register(_ATTENTION, _paged_attention)
+    before = model.config._attn_implementation
+    model.set_attn_implementation(_ATTENTION)
+    _active.cache, _active.cu_tokens = cache, None
+    try:
+        yield
+    finally:
+        model.set_attn_implementation(before)
+        del _active.cache, _active.cu_tokens
+
+
+def cache_for_model(model, max_seqs: int, max_tokens: int, *, page_size: int = 16, num_pages: int | None = None) -> PagedCache:
+    """An empty cache of the model's layers, key heads and dtype for
+    ``max_seqs`` sequences of up to ``max_tokens`` tokens; by default with pages
+    for all of them at once, plus one each for a copy of a shared page."""
+    c = model.config
+    dim = getattr(c, "head_dim", None) or c.hidden_size // c.num_attention_heads
+    width = -(-max_tokens // page_size)
+    p = next(model.parameters())
+    return PagedCache(num_layers=c.num_hidden_layers, num_pages=num_pages or max_seqs * (width + 1),
+                      kv_heads=getattr(c, "num_key_value_heads", None) or c.num_attention_heads, head_dim=dim,
+                      page_size=page_size, max_seqs=max_seqs, max_pages=width, dtype=p.dtype, device=p.device)
+
+
+def _prefill(model, cache: PagedCache, input_ids: torch.Tensor) -> torch.Tensor:
+    """Runs prompts [batch, T] into the cache's first rows; logits of their
+    last positions [batch, vocab]."""
+    batch, new = input_ids.shape
+    n_new = torch.zeros(cache.max_seqs, dtype=torch.int32, device=cache.device)
+    n_new[:batch] = new
+    cache.advance(n_new)
+    cu = torch.zeros(cache.max_seqs + 1, dtype=torch.int32, device=cache.device)
+    cu[1:] = torch.cumsum(n_new, 0)
+    _active.cu_tokens = cu
+    return model(input_ids=input_ids, use_cache=False, logits_to_keep=1).logits[:, -1]
+
+
+def _decode(model, cache: PagedCache, tokens: torch.Tensor) -> torch.Tensor:
+    """One step: tokens [rows] are the last of rows that advance() has just
+    grown by one; their logits [rows, vocab]."""
+    positions = (cache.lens[:tokens.shape[0]] - 1).long()[:, None]
+    return model(input_ids=tokens[:, None], position_ids=positions, use_cache=False).logits[:, -1]
+
+
+def _finite(logprobs: torch.Tensor) -> None:
+    if not torch.isfinite(logprobs).all():
+        raise FloatingPointError("Non-finite inference logits.")
+
+
+@torch.inference_mode()
+def generate_paged(model, input_ids: torch.Tensor, max_new_tokens: int, *, page_size: int = 16) -> torch.Tensor:
+    """:func:`~s_salaad_b200.inference.generate` on a paged cache (same
+    arguments, result and errors; equal greatest logits: the lowest token).
+    Logits are checked once, after the last step."""
+    from .generate import _check_request
+
+    _check_request(model, input_ids, max_new_tokens)
+    if max_new_tokens == 0:
+        return input_ids
+    batch, prompt = input_ids.shape
+    cache = cache_for_model(model, batch, prompt + max_new_tokens, page_size=page_size)
+    chosen, logprobs = [], []
+    with _on_cache(model, cache):
+        logits = _prefill(model, cache, input_ids)
+        for step in range(max_new_tokens):
+            if step:
+                cache.advance(1)
+                logits = _decode(model, cache, chosen[-1])
+            best = token_logprobs(logits, top=1, entropy=False)
+            chosen.append(best.top_ids[:, 0])
+            logprobs.append(best.top_logprobs)
+    _finite(torch.cat(logprobs, dim=1))
+    cache.check()
+    return torch.cat([input_ids, torch.stack(chosen, dim=1)], dim=1)
+
+
+@torch.inference_mode()
+def beam_search(model, input_ids: torch.Tensor, max_new_tokens: int, beams: int, *,
+                page_size: int = 16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Beam search with ``beams`` (1 to 32) hypotheses per prompt of
+    ``input_ids`` [batch, prompt]: (sequences [batch, beams, prompt +
+    max_new_tokens], scores [batch, beams]), the score of a sequence being the
+    sum of its new tokens' log probabilities, best first."""
+    from .generate import _check_request
+
+    _check_request(model, input_ids, max_new_tokens)
+    if max_new_tokens == 0:
+        raise ValueError("beam search needs at least one new token.")
+    vocab = model.config.vocab_size
+    if not 1 <= beams <= min(32, vocab):
+        raise ValueError("beams must be between 1 and min(32, vocabulary).")
+    batch, prompt = input_ids.shape
+    cache = cache_for_model(model, batch * beams, prompt + max_new_tokens, page_size=page_size)
+    dev = cache.device
+    with _on_cache(model, cache):
+        best = token_logprobs(_prefill(model, cache, input_ids), top=beams, entropy=False)
+        scores, tokens = best.top_logprobs, best.top_ids  # [batch, beams]
+        sequences = torch.cat([input_ids[:, None].expand(batch, beams, prompt), tokens[..., None]], dim=2)
+        first_row = torch.arange(batch, device=dev)[:, None] * beams
+        parents = torch.arange(batch, device=dev)[:, None].expand(batch, beams)  # the prompts' rows
+        for _ in range(max_new_tokens - 1):
+            cache.advance(1, parents=parents.reshape(-1).to(torch.int32))
+            best = token_logprobs(_decode(model, cache, tokens.reshape(-1)), top=beams, entropy=False)
+            total = scores.reshape(batch, beams, 1) + best.top_logprobs.view(batch, beams, beams)
+            scores, at = total.view(batch, -1).topk(beams, dim=1)
+            tokens = best.top_ids.view(batch, -1).gather(1, at)
+            parent = at // beams
+            parents = first_row + parent
+            kept = sequences.gather(1, parent[..., None].expand(batch, beams, sequences.shape[2]))
+            sequences = torch.cat([kept, tokens[..., None]], dim=2)
+    _finite(scores)
+    cache.check()
+    return sequences, scores
+
+
+@torch.inference_mode()
+def score(model, input_ids: torch.Tensor, *, top: int = 0, ignore_id: int | None = None) -> TokenLogprobs:
+    """Log probability of every token of ``input_ids`` [batch, length] given
+    the ones before it, entropy, and the ``top`` likeliest tokens in its place:
+    tensors [batch, length - 1] (and [..., top]) for the tokens from the second
+    on.  Targets equal to ``ignore_id`` (padding) get log probability 0."""
+    if input_ids.ndim != 2 or input_ids.shape[1] < 2:
+        raise ValueError("Expected a batch of at least two input token IDs each.")
+    logits = model(input_ids=input_ids, use_cache=False).logits
+    # the last position predicts nothing: scoring it too keeps the rows packed
+    targets = torch.full_like(input_ids, -100)
+    targets[:, :-1] = input_ids[:, 1:]
+    if ignore_id is not None:
+        targets.masked_fill_(targets == ignore_id, -100)
+    r = token_logprobs(logits, targets, top=top)
+    return TokenLogprobs(*(None if t is None else t[:, :-1] for t in r))

@@ -179,6 +179,28 @@ class PagedCache:
         if rc:
             _lib.check(rc, "kv_compact")
 
+    def resize(self, num_pages: int) -> None:
+        """Moves the cache to a new pool of ``num_pages`` pages (more, or after
+        rows have left fewer: the live pages are compacted first).  Waits for
+        the GPU; raises ValueError if the live pages do not fit.  A pool or
+        state given at construction, and graphs captured with this cache, are
+        not used afterwards."""
+        if not 1 <= int(num_pages) < 2 ** 31:
+            raise ValueError(f"num_pages must be in [1, 2^31), got {num_pages}")
+        self.compact()
+        live = int(self.header[3])
+        if live > num_pages:
+            raise ValueError(f"{live} pages are in use, more than {num_pages}")
+        new = PagedCache(num_layers=self.num_layers, num_pages=num_pages, kv_heads=self.kv_heads,
+                         head_dim=self.head_dim, page_size=self.page_size, max_seqs=self.max_seqs,
+                         max_pages=self.max_pages, dtype=self.dtype, device=self.device)
+        new.pool[:, :, :live] = self.pool[:, :, :live]
+        new.header.copy_(self.header)
+        new.lens.copy_(self.lens)
+        new.refs[:live] = self.refs[:live]
+        new.page_table.copy_(self.page_table)
+        self.__dict__.update(new.__dict__)
+
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Copies pages ``src[i]`` to ``dst[i]`` (int32) of every layer; the
         state is not touched.  Pairs that clash (a dst that is another pair's
