@@ -78,16 +78,6 @@ struct Sums {
 // (a - b) log2 e, finite: a product with a sum of 0 stays 0.  The difference
 // is taken first: logits of the type's lowest value times log2 e overflow.
 __device__ __forceinline__ float log2_gap(float a, float b) { return fmaxf((a - b) * kLog2e, -1e30f); }
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-  Sums r;
-  r.m = fmaxf(a.m, b.m);
-  const float da = a.m == -INFINITY ? 0.f : log2_gap(a.m, r.m), db = b.m == -INFINITY ? 0.f : log2_gap(b.m, r.m);
-  const float fa = a.m == -INFINITY ? 0.f : ex2(da), fb = b.m == -INFINITY ? 0.f : ex2(db);
-  r.s = a.s * fa + b.s * fb;
-  r.u = fa * (a.u + a.s * da) + fb * (b.u + b.s * db);
-  return r;
-}
-
 // Unique key of element i: greater for a greater value, then for a lower
 // index.  NaN ranks with -inf; -0 with +0.
 __device__ __forceinline__ unsigned long long key_of(float x, uint32_t i) {
@@ -499,9 +489,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   }
   if (parts > 1) cluster.sync();
   else __syncthreads();
-  if (part == 0 && w == 0) {
-    Sums all = sh.mine;
-    for (int p = 1; p < parts; ++p) all = join(all, *cluster.map_shared_rank(&sh.mine, p));
+  if (part == 0) {
+    // the parts' lists, merged pairwise by one warp each
+    Key list = 0ull;
+    if (k) {
+      int n = parts;
+      if (w < (n + 1) / 2) list = cluster.map_shared_rank(sh.best, w)[lane];
+      if (n > 1 && w < n / 2) list = warp_merge(list, cluster.map_shared_rank(sh.best, w + n / 2)[31 - lane]);
+      for (n /= 2; n > 1; n /= 2) {
+        if (w >= n / 2 && w < n) sh.lists[w][lane] = list;
+        __syncthreads();
+        if (w < n / 2) list = warp_merge(list, sh.lists[w + n / 2][31 - lane]);
+      }
+    }
+  if (w == 0) {
+    const Sums all =
+        parts == 1 ? sh.mine
+                   : warp_join(lane < parts ? *cluster.map_shared_rank(&sh.mine, lane) : Sums{-INFINITY, 0.f, 0.f});
     const float log_s = log2f(all.s);
     const bool none = !(all.s > 0.f);  // no finite logit, or a NaN
     const float nan = __int_as_float(0x7fffffff);
@@ -515,13 +519,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       }
     }
     if (k) {
-      Key list = sh.best[lane];
-      for (int p = 1; p < parts; ++p) list = warp_merge(list, cluster.map_shared_rank(sh.best, p)[31 - lane]);
       if (lane < k) {
         a.top_ids[r * k + lane] = int64_t(0xffffffffu - uint32_t(list));
         a.top_logprobs[r * k + lane] = logprob(value_of(list));
       }
     }
+  }
   }
   if (parts > 1) cluster.sync();  // the parts stay until they have been read
 }

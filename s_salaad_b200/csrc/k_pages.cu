@@ -31,80 +31,118 @@ struct PagesK {
   int32_t *growers, *first, *list, *src, *dst;  // workspace
 };
 
-__device__ __forceinline__ int64_t pages_of(int64_t len, int page_size) { return (len + page_size - 1) / page_size; }
+__device__ __forceinline__ int64_t pages_of(int64_t len, int page_size) {
+  if (len < (int64_t(1) << 31)) return (uint32_t(len) + uint32_t(page_size) - 1) / uint32_t(page_size);  // short division
+  return (len + page_size - 1) / page_size;
+}
 
-// Length of row r after the selection and before growth, clipped to the table.
-__device__ __forceinline__ int64_t kept_length(const PagesK& p, const int32_t* parents, const int32_t* n_new, int n_all,
-                                               int r, bool* bad) {
-  int from = parents ? parents[r] : r;
-  if (from >= p.rows) {
-    *bad = true;
-    from = -1;
-  }
-  if (from < 0) return 0;
-  int64_t len = p.lens[from];
+// Length of a row after a change by n < 0 (before any growth).
+__device__ __forceinline__ int kept_length(int len, int64_t n) {
+  return int(n < 0 ? (len + n < 0 ? 0 : len + n) : len);
+}
+
+// A row's length as the state has it, clipped to the table.
+__device__ __forceinline__ int checked_length(const PagesK& p, int r, bool* bad) {
   const int64_t cap = int64_t(p.max_pages) * p.page_size;
+  const int len = p.lens[r];
   if (len < 0 || len > cap) {
     *bad = true;
-    len = len < 0 ? 0 : cap;
+    return int(len < 0 ? 0 : cap);
   }
-  const int64_t n = n_new ? n_new[r] : n_all;
-  return n < 0 ? (len + n < 0 ? 0 : len + n) : len;
+  return len;
+}
+
+// The row that row r becomes a copy of; -1: empty.
+__device__ __forceinline__ int checked_parent(const PagesK& p, const int32_t* parents, int r, bool* bad) {
+  const int from = parents ? parents[r] : r;
+  if (from >= p.rows) *bad = true;
+  return from >= p.rows || from < 0 ? -1 : from;
 }
 
 // Table rows become their parents' rows, entries behind the kept length -1.
 // Columns are independent, so a CTA reads its kCols columns of every row
 // before it writes them: in place, one launch.  refs follow by integer
-// atomics; each CTA adds its change of the number of live pages.  Bound by the
-// atomics' latency: few columns per CTA (32 took 54 us for 250 rows x 120
-// pages, 4 take 6).
+// atomics, per parent: its pages gain (children - 1) references, nothing where
+// a row merely moves, and each child loses those behind its kept length.  Each
+// CTA adds its change of the number of live pages.  Bound by latency: few
+// columns per CTA, everything read at once (250 rows x 120 pages: 32 columns
+// and two atomics per entry took 54 us, 4 columns 11).
 constexpr int kCols = 4;
+constexpr int kEarly = 4;  // entries that a thread reads before the lengths are known
 __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32_t* parents, const int32_t* n_new,
                                                      int n_all) {
   extern __shared__ int32_t sm[];
   int32_t* old = sm;                     // [rows][kCols]
-  int32_t* keep = old + p.rows * kCols;  // [rows] entries kept
-  int32_t* from = keep + p.rows;         // [rows]
+  int32_t* len = old + p.rows * kCols;   // [rows] lengths before
+  int32_t* from = len + p.rows;          // [rows]
+  int32_t* children = from + p.rows;     // [rows]
   __shared__ int s_most, s_live;
   const int tid = threadIdx.x, c0 = blockIdx.x * kCols;
   pdl_wait_primary();
   pdl_launch_dependents();
+  auto entry = [&](int i) {
+    const int c = c0 + i % kCols;
+    return c < p.max_pages ? p.table[int64_t(i / kCols) * p.max_pages + c] : -1;
+  };
+  int early[kEarly];
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int i = k * int(blockDim.x) + tid;
+    early[k] = i < p.rows * kCols ? entry(i) : -1;
+  }
   if (tid == 0) s_most = 0, s_live = 0;
-  __syncthreads();
   bool bad = false;
   int most = 0;
   for (int r = tid; r < p.rows; r += blockDim.x) {
-    keep[r] = int(pages_of(kept_length(p, parents, n_new, n_all, r, &bad), p.page_size));
-    const int f = parents ? parents[r] : r;
-    from[r] = f >= p.rows ? -1 : f;
-    const int64_t len = p.lens[r];
-    most = max(most, int(min(int64_t(p.max_pages), pages_of(max(len, int64_t(0)), p.page_size))));
+    from[r] = checked_parent(p, parents, r, &bad);
+    len[r] = checked_length(p, r, &bad);
+    children[r] = 0;
+    most = max(most, len[r]);
   }
+  __syncthreads();
   most = __reduce_max_sync(0xffffffffu, most);
   if ((tid & 31) == 0) atomicMax(&s_most, most);
+  for (int r = tid; r < p.rows; r += blockDim.x)
+    if (from[r] >= 0) atomicAdd(children + from[r], 1);
   if (bad && blockIdx.x == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
-  __syncthreads();
-  // no row has an entry from here on: there is nothing to move or to drop
-  if (c0 >= s_most) return;
-#pragma unroll 4
-  for (int i = tid; i < p.rows * kCols; i += blockDim.x) {
-    const int c = c0 + i % kCols;
-    old[i] = c < p.max_pages ? p.table[int64_t(i / kCols) * p.max_pages + c] : -1;
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int i = k * int(blockDim.x) + tid;
+    if (i < p.rows * kCols) old[i] = early[k];
   }
   __syncthreads();
-  int live = 0;
+  // no row has an entry from here on: there is nothing to move or to drop
+  if (c0 >= pages_of(s_most, p.page_size)) return;
 #pragma unroll 4
+  for (int i = kEarly * int(blockDim.x) + tid; i < p.rows * kCols; i += blockDim.x) old[i] = entry(i);
+  __syncthreads();
+  int live = 0;
+  auto refer = [&](int page, int change) {
+    if (page < 0) return;
+    if (page >= p.num_pages) {
+      atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
+      return;
+    }
+    // a page is live while its count is above 0: the crossings add up to the net change
+    const int was = atomicAdd(p.refs + page, change);
+    live += int(was + change > 0) - int(was > 0);
+  };
+#pragma unroll 2
   for (int i = tid; i < p.rows * kCols; i += blockDim.x) {
     const int r = i / kCols, j = i % kCols, c = c0 + j;
     if (c >= p.max_pages) continue;
-    const int was = old[i];
-    const int now = from[r] >= 0 && c < keep[r] ? old[from[r] * kCols + j] : -1;
-    if (was == now) continue;
-    p.table[int64_t(r) * p.max_pages + c] = now;
-    if (was >= p.num_pages || now >= p.num_pages) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
-    // a page is live while its count is above 0: the crossings add up to the net change
-    if (now >= 0 && now < p.num_pages) live += atomicAdd(p.refs + now, 1) == 0;
-    if (was >= 0 && was < p.num_pages) live -= atomicAdd(p.refs + was, -1) == 1;
+    const int was = old[i], f = from[r];
+    if (children[r] != 1) refer(was, children[r] - 1);
+    int now = -1;
+    if (f >= 0) {
+      now = old[f * kCols + j];
+      const int keep = kept_length(len[f], n_new ? n_new[r] : n_all);
+      if (c >= pages_of(keep, p.page_size)) {
+        refer(now, -1);
+        now = -1;
+      }
+    }
+    if (was != now) p.table[int64_t(r) * p.max_pages + c] = now;
   }
   live = __reduce_add_sync(0xffffffffu, live);
   if ((tid & 31) == 0 && live) atomicAdd(&s_live, live);
@@ -113,6 +151,7 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
 }
 
 constexpr int kGrowThreads = 1024;
+constexpr int kListed = 2048;  // pages given out in one call that are listed in shared memory
 constexpr int kPer = 8;  // pages of a thread in one step of a scan over refs
 
 // Exclusive scan over the block; *total: the sum.  `sums`: 32 words of shared
@@ -160,7 +199,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
   int32_t* copy = start + p.rows + 1;
   __shared__ int64_t sums64[32];
   __shared__ int sums[32];
-  __shared__ int s_over;
+  __shared__ int s_over, s_list[kListed];
   const int tid = threadIdx.x;
   pdl_wait_primary();
   pdl_launch_dependents();
@@ -172,7 +211,16 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     const int64_t n = n_new ? n_new[r] : n_all;
     return n <= 0 || (!n_new && low[r] == 0) ? 0 : n;  // one number for all: rows that hold tokens
   };
-  for (int r = tid; r < p.rows; r += kGrowThreads) low[r] = int(kept_length(p, parents, n_new, n_all, r, &bad));
+  // lens and parents are read side by side; start holds the lengths before for a moment
+  for (int r = tid; r < p.rows; r += kGrowThreads) {
+    copy[r] = checked_parent(p, parents, r, &bad);
+    start[r] = checked_length(p, r, &bad);
+  }
+  __syncthreads();
+  for (int r = tid; r < p.rows; r += kGrowThreads) {
+    const int from = copy[r];
+    low[r] = from < 0 ? 0 : kept_length(start[from], n_new ? n_new[r] : n_all);
+  }
   __syncthreads();
   // rows about to write into a shared last page
   auto shared_last = [&](int r) -> int {
@@ -232,7 +280,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
       if (fits && k < total)
         for (int j = 0; j < kPer; ++j)
           if (mask >> j & 1u) {
-            if (k < total) p.list[k] = int32_t(i0 + j);
+            if (k < total) (k < kListed ? s_list[k] : p.list[k]) = int32_t(i0 + j);
             ++k;
           }
       found += sum;
@@ -249,7 +297,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
         if (start[mid] <= k) lo = mid;
         else hi = mid - 1;
       }
-      const int r = lo, page = p.list[k];
+      const int r = lo, page = k < kListed ? s_list[k] : p.list[k];
       int j = k - start[r] - (copy[r] >= 0 ? 1 : 0);
       const int64_t col = pages_of(low[r], p.page_size) + j;  // j == -1: the copied page
       p.table[int64_t(r) * p.max_pages + col] = page;
@@ -262,7 +310,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     for (int r = r0; r < r1; ++r)
       if (copy[r] >= 0) {
         p.src[c] = copy[r];
-        p.dst[c] = p.list[start[r]];
+        p.dst[c] = start[r] < kListed ? s_list[start[r]] : p.list[start[r]];
         ++c;
         atomicAdd(p.refs + copy[r], -1);  // another row keeps it
       }
@@ -509,7 +557,7 @@ int prepare_device(int* sms) {
   int n = dev < kDevices ? known[dev].load(std::memory_order_acquire) : 0;
   if (!n) {
     SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        kAttendMaxRows * (kCols + 2) * 4));
+                                        kAttendMaxRows * (kCols + 3) * 4));
     SLR_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
     if (dev < kDevices) known[dev].store(n, std::memory_order_release);
   }
@@ -562,7 +610,7 @@ int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const
   int rc = prepare_device(&sms);
   if (rc) return rc;
   if (parents || n_new || n_all < 0) {
-    const size_t smem = size_t(p.rows) * (kCols + 2) * 4;
+    const size_t smem = size_t(p.rows) * (kCols + 3) * 4;
     rc = launch_after(select_kernel, dim3(unsigned(ceil_div(p.max_pages, kCols))), 256, smem, s, k, parents,
                                 n_new, n_all);
     if (rc) return rc;

@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _DeviceGuard, _no_graph, _require_cuda, _stream, slr_dtype
+from .ops import _DeviceGuard, _no_graph, _require_cuda, _stream, _switch, slr_dtype
 
 HEADER = _lib.SLR_KV_HEADER_WORDS
 
@@ -162,10 +162,14 @@ class PagedCache:
                 raise ValueError(f"n_new out of range: {n_all}")
         if parents is not None:
             parents = self._vector("parents", parents, self.max_seqs)
-        with _DeviceGuard(self.device):
+        back = _switch(self._index)
+        try:
             ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=self.device)
             rc = self._lib.slr_kv_advance(self._ref, None if parents is None else parents.data_ptr(), n_ptr, n_all,
                                           ws.data_ptr(), self._pages_ws, _stream(self.device))
+        finally:
+            if back >= 0:
+                torch.cuda.set_device(back)
         if rc:
             _lib.check(rc, "kv_advance")
 
@@ -173,9 +177,13 @@ class PagedCache:
         """Moves the live pages to the lowest numbers (order kept among the
         moved ones) and rewrites the table; the pages from ``header[3]`` on are
         free then."""
-        with _DeviceGuard(self.device):
+        back = _switch(self._index)
+        try:
             ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=self.device)
             rc = self._lib.slr_kv_compact(self._ref, ws.data_ptr(), self._pages_ws, _stream(self.device))
+        finally:
+            if back >= 0:
+                torch.cuda.set_device(back)
         if rc:
             _lib.check(rc, "kv_compact")
 
@@ -259,9 +267,13 @@ class PagedCache:
         if cu_tokens is not None:
             cu_tokens = self._vector("cu_tokens", cu_tokens, self.max_seqs + 1)
             cu = cu_tokens.data_ptr()
-        with _DeviceGuard(self.device):
+        back = _switch(self._index)
+        try:
             rc = self._lib.slr_kv_append(self._ref, layer, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
                                          shape[0], cu, _stream(self.device))
+        finally:
+            if back >= 0:
+                torch.cuda.set_device(back)
         if rc:
             _lib.check(rc, "kv_append")
 
@@ -286,7 +298,8 @@ class PagedCache:
             if out_shape != shape:
                 raise ValueError(f"out must be {tuple(shape)}, got {tuple(out_shape)}")
         lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device) if return_lse else None
-        with _DeviceGuard(self.device):
+        back = _switch(self._index)
+        try:
             need = self._attend_ws.get((rows, heads))
             if need is None:
                 need = int(self._lib.slr_kv_attend_workspace_size(self._ref, rows, heads))
@@ -298,6 +311,9 @@ class PagedCache:
                 self._ref, layer, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
                 lse.data_ptr() if return_lse else None, rows, heads, dim ** -0.5 if scale is None else scale,
                 ws, need, _stream(self.device))
+        finally:
+            if back >= 0:
+                torch.cuda.set_device(back)
         if rc:
             _lib.check(rc, "kv_attend")
         return (out, lse) if return_lse else out

@@ -45,6 +45,16 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _switch(index: int) -> int:
+    """Make device `index` current; returns the one to go back to, or -1 (the
+    cheap form of _DeviceGuard, for calls of a few microseconds)."""
+    current = torch.cuda.current_device()
+    if current == index:
+        return -1
+    torch.cuda.set_device(index)
+    return current
+
+
 def _require_cuda(name: str, t: torch.Tensor) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (s_salaad_b200 has no CPU path)")
@@ -722,12 +732,16 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     if top:
         ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
         val = torch.empty(rows, top, dtype=torch.float32, device=dev)
-    with _DeviceGuard(dev):
+    back = _switch(dev.index)
+    try:
         rc = _lib.load().slr_token_logprobs(
             x.data_ptr(), stride if rows > 1 else vocab, rows, vocab, dtype,
             None if lp is None else targets.data_ptr(), None if lp is None else lp.data_ptr(),
             None if ent is None else ent.data_ptr(), top, None if ids is None else ids.data_ptr(),
             None if val is None else val.data_ptr(), _stream(dev))
+    finally:
+        if back >= 0:
+            torch.cuda.set_device(back)
     if rc:
         _lib.check(rc, "token_logprobs")
     if len(full) != 2:
