@@ -95,12 +95,12 @@ using Key = unsigned long long;
 __device__ __forceinline__ Key max_key(Key a, Key b) { return a > b ? a : b; }
 
 // Bitonic networks over a warp's 32 keys (one per lane), greatest first.
-__device__ __forceinline__ Key merge_step(Key k, int j, bool descending) {
-  const Key other = __shfl_xor_sync(0xffffffffu, k, j);
+template <typename K> __device__ __forceinline__ K merge_step(K k, int j, bool descending) {
+  const K other = __shfl_xor_sync(0xffffffffu, k, j);
   const bool low_lane = ((threadIdx.x & 31) & j) == 0;
-  return (low_lane == descending) == (k > other) ? k : other;
+  return low_lane == descending ? max(k, other) : min(k, other);
 }
-__device__ __forceinline__ Key warp_sort(Key k) {
+__device__ __forceinline__ uint32_t warp_sort(uint32_t k) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
@@ -109,11 +109,26 @@ __device__ __forceinline__ Key warp_sort(Key k) {
   return k;
 }
 // The 32 greatest of two sorted lists, sorted: a's lane i against b's lane 31 - i.
-__device__ __forceinline__ Key warp_merge(Key a, Key b_reversed) {
-  Key k = max_key(a, b_reversed);
+template <typename K> __device__ __forceinline__ K warp_merge(K a, K b_reversed) {
+  K k = max(a, b_reversed);
 #pragma unroll
   for (int j = 16; j; j >>= 1) k = merge_step(k, j, true);
   return k;
+}
+
+// Room for `count` entries of every lane behind *counter (shared memory, one
+// atomic per warp): this lane's first.
+__device__ __forceinline__ int warp_reserve(int count, int* counter) {
+  const int lane = threadIdx.x & 31;
+  int incl = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  int base = 0;
+  if (lane == 31 && incl) base = atomicAdd(counter, incl);
+  return __shfl_sync(0xffffffffu, base, 31) + incl - count;
 }
 
 template <typename T> struct Vec;
@@ -200,7 +215,7 @@ template <typename T> struct Shared {
   Key cand[kCandidates];
   Key best[32];       // this CTA's list, greatest first
   Sums mine;
-  Key tau, next;
+  uint32_t values[32], tau_value, tau_index[2];
   int n_cand, n_elig;
   T group[kGroups<T>][kThreads];      // greatest value of each thread's groups of batches
   unsigned short elig[kEligible];  // groups to read again
@@ -384,46 +399,56 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   const int k = a.top;
   if (k) {
     const bool has = best_last >= 0;
-    // 64 sets of two threads: sorted by two warps, merged by one
+    // 64 sets of two threads: their values sorted by two warps, merged by one
     const Key own = has ? key_of(best, best_last) : 0ull;
     if (w >= 2) sh.lists[w - 2][lane] = own;
     __syncthreads();
     if (w < 2) {
-      const Key mine = warp_sort(max_key(own, sh.lists[w][lane]));
-      if (w == 1) sh.lists[1][lane] = mine;
+      const Key set = max_key(own, sh.lists[w][lane]);
+      const uint32_t value = uint32_t(set >> 32), sorted = warp_sort(value);
+      if (w == 1) sh.values[lane] = sorted;
       named_bar_sync(1, 64);
       if (w == 0) {
-        const Key both = warp_merge(mine, sh.lists[1][31 - lane]);
-        if (lane == k - 1) sh.tau = both;  // 0 when fewer than k sets have elements: all are candidates
+        const uint32_t both = warp_merge(sorted, sh.values[31 - lane]);
+        if (lane == k - 1) sh.tau_value = both;  // 0 when fewer than k sets have elements: all are candidates
       }
+      named_bar_sync(1, 64);
+      // of equal values the highest index: all of these sets count
+      const bool equal = value == sh.tau_value;
+      const uint32_t low = __reduce_min_sync(0xffffffffu, equal ? uint32_t(set) : 0xffffffffu);
+      if (lane == 0) sh.tau_index[w] = low;
     }
     __syncthreads();
-    const Key tau = sh.tau;
+    const Key tau =
+        sh.tau_value ? static_cast<Key>(sh.tau_value) << 32 | min(sh.tau_index[0], sh.tau_index[1]) : 0ull;
     const float tau_x = tau ? value_of(tau) : -INFINITY;
     const int groups = (n_batch + (1 << group_log) - 1) >> group_log;
-    for (int g = 0; g < groups; ++g)
-      if (to_f(sh.group[g][tid]) >= tau_x) {
-        const int at = atomicAdd(&sh.n_elig, 1);
-        if (at < kEligible) sh.elig[at] = static_cast<unsigned short>(g * kThreads + tid);
-      }
+    {
+      unsigned long long mask = 0;
+      for (int g = 0; g < groups; ++g)
+        if (to_f(sh.group[g][tid]) >= tau_x) mask |= 1ull << g;
+      int at = warp_reserve(__popcll(mask), &sh.n_elig);
+      for (; mask; mask &= mask - 1, ++at)
+        if (at < kEligible) sh.elig[at] = static_cast<unsigned short>((__ffsll(mask) - 1) * kThreads + tid);
+    }
     __syncthreads();
-    auto offer = [&](Key key) {
-      if (key < tau) return;
-      const int at = atomicAdd(&sh.n_cand, 1);
-      if (at < kCandidates) sh.cand[at] = key;
+    // whether an element is a candidate (NaN counts as -inf)
+    auto passes = [&](float x, int i) {
+      const float y = x == x ? x : -INFINITY;
+      return y > tau_x || (y == tau_x && key_of(y, i) >= tau);
     };
     // four reads in flight per thread: the latency of DRAM counts here
     const int sub_log = group_log + 2;
     const bool all = sh.n_elig > kEligible;  // many equal values: every vector
     const int items = all ? v1 - v0 : sh.n_elig << sub_log;
-    for (int q0 = tid; q0 < items; q0 += 4 * kThreads) {
+    for (int q0 = tid; q0 - lane < items; q0 += 4 * kThreads) {
       uint4 v[4];
       int at[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int q = q0 + i * kThreads;
         at[i] = v1;
-        if (all) {
+        if (q < items && all) {
           at[i] = v0 + q;
         } else if (q < items) {
           const int e = sh.elig[q >> sub_log];
@@ -431,6 +456,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
         }
         if (at[i] < v1) v[i] = row.load(at[i]);
       }
+      unsigned mask = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (at[i] >= v1 || V::of_top(V::top(v[i])) < tau_x) continue;  // all NaN goes on
@@ -438,10 +464,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
         V::to_floats(v[i], x);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (!(x[e] < tau_x)) offer(key_of(x[e], row.first_of(at[i]) + e));
+          if (passes(x[e], row.first_of(at[i]) + e)) mask |= 1u << (i * E + e);
       }
+      __syncwarp();
+      int to = warp_reserve(__popc(mask), &sh.n_cand);
+      for (; mask; mask &= mask - 1, ++to) {
+        const int b = __ffs(mask) - 1, i = b / E;
+        const int idx = row.first_of(i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3]) + b % E;
+        if (to < kCandidates) sh.cand[to] = key_of(to_f(row.x[idx]), idx);
+      }
+      __syncwarp();
     }
-    if (edge) offer(key_of(edge_x, row.edge(tid)));
+    if (edge && passes(edge_x, row.edge(tid))) {
+      const int to = atomicAdd(&sh.n_cand, 1);
+      if (to < kCandidates) sh.cand[to] = key_of(edge_x, row.edge(tid));
+    }
     __syncthreads();
     const int n = sh.n_cand;
     if (n <= kCandidates) {

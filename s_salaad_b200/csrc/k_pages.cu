@@ -404,6 +404,10 @@ struct CopyK {
 
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;
+// CTAs per SM of a copy that is known to be long: dealt by the hardware as SMs
+// come free (6000 pages, 3/5 live: 8 per SM, each with a fixed share, 275 us,
+// 24: 258, 64: 252).  Copies that are mostly empty keep to one wave of 8.
+constexpr int kManyCtas = 64;
 
 template <int V> struct vec_of;
 template <> struct vec_of<16> { using type = uint4; };
@@ -467,14 +471,15 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyK a) {
   }
 }
 
+constexpr int kAppendThreads = 64;  // 48k tokens of 8 heads of 128: 35.9 us, with 128 threads 36.6, with 512 41.5
 // New tokens into their pages: one warp per token, 16-byte chunks (V = 16) or
 // single elements where the caller's rows are not aligned (V = element size).
 template <int V>
-__global__ void __launch_bounds__(128) append_kernel(const AppendArgs a, int esize) {
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a, int esize) {
   pdl_wait_primary();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
-  const int64_t token = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int64_t token = int64_t(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
   if (token >= a.tokens) return;
   int row = int(token);
   int64_t pos;
@@ -585,7 +590,7 @@ PagesK views(const PagesArgs& p) {
   return k;
 }
 
-int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, int sms, cudaStream_t s) {
+int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, int64_t ctas, cudaStream_t s) {
   c.k = p.k;
   c.v = p.v;
   c.layer_bytes = p.layer_bytes;
@@ -595,7 +600,7 @@ int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, int sms, cudaSt
   c.num_pages = p.num_pages;
   const int64_t pieces = ceil_div(p.page_bytes, int64_t(kCopyThreads) * kCopyUnroll * 16);
   const int64_t items = std::max<int64_t>(1, pieces * c.planes * most_pairs);
-  return launch_after(copy_kernel<16>, dim3(unsigned(std::min<int64_t>(items, int64_t(sms) * 8))), kCopyThreads, 0, s, c);
+  return launch_after(copy_kernel<16>, dim3(unsigned(std::min(items, ctas))), kCopyThreads, 0, s, c);
 }
 
 }  // namespace
@@ -622,7 +627,7 @@ int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const
   c.src = k.src;
   c.dst = k.dst;
   c.count = k.head + kCopies;
-  return copy_launch(p, c, p.rows, sms, s);
+  return copy_launch(p, c, p.rows, 8 * sms, s);
 }
 
 int launch_kv_compact(const PagesArgs& p, cudaStream_t s) {
@@ -640,7 +645,8 @@ int launch_kv_compact(const PagesArgs& p, cudaStream_t s) {
   c.to = k.first;
   c.live = k.head + kLive;
   c.entries = int64_t(p.rows) * p.max_pages;
-  return copy_launch(p, c, std::max<int64_t>(p.num_pages / 2, ceil_div(c.entries, 1024)), sms, s);
+  return copy_launch(p, c, std::max<int64_t>(p.num_pages / 2, ceil_div(c.entries, 1024)),
+                     kManyCtas * sms, s);
 }
 
 int launch_kv_copy(const PagesArgs& p, const int32_t* src, const int32_t* dst, int n, cudaStream_t s) {
@@ -652,7 +658,7 @@ int launch_kv_copy(const PagesArgs& p, const int32_t* src, const int32_t* dst, i
   c.dst = dst;
   c.n = n;
   c.check = true;
-  return copy_launch(p, c, n, sms, s);
+  return copy_launch(p, c, n, kManyCtas * sms, s);
 }
 
 int launch_kv_append(const AppendArgs& a, cudaStream_t s) {
@@ -660,10 +666,10 @@ int launch_kv_append(const AppendArgs& a, cudaStream_t s) {
   const auto even = [&](int64_t stride) { return stride * e % 16 == 0; };
   const bool wide = aligned16(a.new_k) && aligned16(a.new_v) && even(a.k_row) && even(a.k_head) && even(a.v_row) &&
                     even(a.v_head) && a.dim * e % 16 == 0;
-  const dim3 grid(unsigned(ceil_div(a.tokens, 4)));
-  if (wide) return launch_after(append_kernel<16>, grid, 128, 0, s, a, e);
-  if (e == 4) return launch_after(append_kernel<4>, grid, 128, 0, s, a, e);
-  return launch_after(append_kernel<2>, grid, 128, 0, s, a, e);
+  const dim3 grid(unsigned(ceil_div(a.tokens, kAppendThreads / 32)));
+  if (wide) return launch_after(append_kernel<16>, grid, kAppendThreads, 0, s, a, e);
+  if (e == 4) return launch_after(append_kernel<4>, grid, kAppendThreads, 0, s, a, e);
+  return launch_after(append_kernel<2>, grid, kAppendThreads, 0, s, a, e);
 }
 
 int read_and_clear_status_pages(unsigned* out) {
