@@ -116,14 +116,16 @@ template <> struct pair_of<__half> {
 };
 
 // Shape of one instance: DP head dimension padded to a power of two, GT query
-// heads per warp, W warps, TT tokens per tile, NS stages per warp.  Two CTAs
-// of 96 KB at DP = 128: 128 KB of loads in flight per SM.
+// heads per warp, W warps, TT tokens per tile, NS stages per warp.  DP = 128: 3
+// CTAs of 64 KB, two stages per warp (2 x 131071 tokens, fp16: 152.6 us; 2 CTAs
+// with three stages 158.5); DP = 64: four stages of 4 KB (12000 tokens, bf16: 98
+// us, three 104.5, six 115).
 template <typename T, int DP_, int GT_> struct Cfg {
   static constexpr bool kF32 = std::is_same<T, float>::value;
   static constexpr int DP = DP_, GT = GT_;
   static constexpr int W = 4;
   static constexpr int TT = kF32 ? 8 : 16;
-  static constexpr int NS = kF32 && GT == 8 ? 2 : DP == 64 ? 4 : 3;
+  static constexpr int NS = DP == 64 && !(kF32 && GT == 8) ? 4 : 2;
   static constexpr int kRow = DP * int(sizeof(T));     // bytes of a token's row
   static constexpr int kHalf = TT * kRow;              // K (or V) bytes of a stage
   static constexpr int kStage = 2 * kHalf;
@@ -406,9 +408,15 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
           to32[i] = v.x, to32[i + 1] = v.y, to32[i + 2] = v.z, to32[i + 3] = v.w;
         }
       } else {
-        for (int i = lane; i < GT * DP; i += 32) {
-          const int g = i / DP, d = i % DP;
-          qs[i] = g < heads && d < a.dim ? q[g * a.q_head + d] : 0.f;
+#pragma unroll
+        for (int i = 0; i < GT * DP / 128; ++i) {
+          const int at = i * 128 + lane * 4, g = at / DP, d = at % DP;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (g < heads && d < a.dim) {  // head_dim is a multiple of 8
+            const float* p = q + g * a.q_head + d;
+            v = a.q_wide ? *reinterpret_cast<const float4*>(p) : make_float4(p[0], p[1], p[2], p[3]);
+          }
+          *reinterpret_cast<float4*>(qs + at) = v;
         }
         __syncwarp();
       }
