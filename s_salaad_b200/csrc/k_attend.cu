@@ -42,7 +42,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kMinTokens = 64;
+// A warp takes at least this many places.  One row of 512 tokens, 8 key heads of
+// 128, bf16: 2 places 10.4 us, 4: 11.9, 1: 9.5, but then 16000 tokens of one key
+// head are 1000 parts to join: 18.2 us, 2: 14.5.
+constexpr int kMinTiles = 2;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -135,7 +138,6 @@ template <typename T, int DP_, int GT_> struct Cfg {
   static constexpr int kP = kF32 ? W * TT * GT * 4 : 0;
   static constexpr int kCnt = W * NS * 4;
   static constexpr int kFixed = kRing + kQ + kP + kCnt + 64 + GT * 8;
-  static constexpr int kMinTiles = kMinTokens / TT;
 };
 
 // Place in the list of tiles: row b, head block h, tile of the row.
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     total += scratch[i];
   }
   const int64_t n_all = int64_t(total) * hb;
-  const int64_t per = tiles_per_worker(n_all, a.workers, C::kMinTiles);
+  const int64_t per = tiles_per_worker(n_all, a.workers, kMinTiles);
   for (int r = r0; r < r1; ++r) {
     if (blockIdx.x == 0) a.prefix[r] = before;
     const int nt = places((lens[r] + TT - 1) / TT);
@@ -835,7 +837,7 @@ __global__ void __launch_bounds__(1024) attend_join_kernel(const AttendK a, int 
   const int kvh = head / a.group, hg = head % a.group, h = kvh * a.hblocks + hg / GT, g = hg % GT;
   pdl_wait_primary();
   const int p0 = a.prefix[b], p1 = a.prefix[b + 1];
-  const int64_t per = tiles_per_worker(int64_t(a.prefix[a.rows]) * hb, a.workers, C::kMinTiles);
+  const int64_t per = tiles_per_worker(int64_t(a.prefix[a.rows]) * hb, a.workers, kMinTiles);
   const int tiles = in && p1 > p0 ? p1 - p0 - kEndCost : 0;
   const int64_t t0 = int64_t(p0) * hb + int64_t(h) * places(tiles), t1 = t0 + tiles;
   const int c0 = tiles ? int(t0 / per) : 0, c1 = tiles ? int((t1 - 1) / per) : 0;
@@ -1015,7 +1017,7 @@ struct Inst {
   }
   // No more warps than shares of tiles that rows of the greatest length could have.
   static int useful(int workers, int rows, int hb, int64_t longest) {
-    const int64_t most = int64_t(rows) * hb * ceil_div(longest, int64_t(C::TT) * C::kMinTiles);
+    const int64_t most = int64_t(rows) * hb * ceil_div(longest, int64_t(C::TT) * kMinTiles);
     return most < workers ? int(round_up(std::max<int64_t>(most, 1), C::W)) : workers;
   }
   static size_t need(int workers, int rows) {
