@@ -39,7 +39,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int, *, paged: bool
     forward per new token, as in the reference: the prompt (with the cache
     filled), then each chosen token alone with the cache.  ``paged`` keeps the
     keys and values in a :class:`~s_salaad_b200.kvcache.PagedCache` and attends
-    with its kernel, instead of the model's own growing cache."""
+    with its kernel, instead of the model's own growing cache (a CUDA model
+    without sliding windows, batches of up to 2048)."""
     if paged:
         from .paged import generate_paged
 

@@ -82,12 +82,10 @@ class PagedCache:
             if tuple(state.shape) != (words,) or not state.is_contiguous():
                 raise ValueError(f"state must be a contiguous vector of {words} words")
         given = [t.device for t in (pool, state) if t is not None]
-        if given:
-            device = given[0]
-        elif device.index is None:
-            device = torch.device("cuda", torch.cuda.current_device())
+        if device.index is None:
+            device = given[0] if given else torch.device("cuda", torch.cuda.current_device())
         if any(d != device for d in given):
-            raise ValueError("pool and state must be on one device")
+            raise ValueError(f"pool and state must be on {device}")
         self.device, self.dtype = device, dtype
         self.num_layers, self.num_pages, self.kv_heads, self.head_dim = num_layers, num_pages, kv_heads, head_dim
         self.page_size, self.max_seqs, self.max_pages = page_size, max_seqs, max_pages
@@ -255,8 +253,8 @@ class PagedCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, cu_tokens: torch.Tensor | None = None) -> None:
         """Writes new tokens' keys and values [tokens, kv_heads, head_dim]
-        into ``layer``, after :meth:`advance` made room: a row's tokens go to
-        its last positions.  ``cu_tokens`` (int32 [max_seqs + 1]): row b's
+        into ``layer``, after :meth:`advance` made room (and gave the row its
+        own copy of a shared last page): a row's tokens go to its last positions.  ``cu_tokens`` (int32 [max_seqs + 1]): row b's
         tokens are ``[cu[b], cu[b + 1])``, further ones are padding.  Without
         it token i is row i's, and empty rows are skipped."""
         shape, ks = self._tokens("k", k)

@@ -317,6 +317,24 @@ def test_two_streams_and_a_graph(cuda):
                 assert not bool(o[r].any())
 
 
+def test_output_in_place_of_q(cuda):
+    """q is read before its row's output is written, in one launch and split."""
+    for width in (None, 5000):
+        cache, k, v = filled_cache([300, 5, 0, 77], kv_heads=2, dim=64, page=16, width=width)
+        q = _q(4, 6, 64, BF16)
+        want = cache.attend(0, q)
+        got = q.clone()
+        assert cache.attend(0, got, out=got) is got and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_q_for_all_rows_and_heads(cuda, dtype):
+    cache, k, v = filled_cache([300, 5, 40], kv_heads=2, dim=64, page=16, dtype=dtype)
+    q = _q(1, 1, 64, dtype).expand(3, 4, 64)
+    assert torch.equal(cache.attend(0, q), cache.attend(0, q.contiguous()))
+    _check(cache, k, v, q, None)
+
+
 def test_refusals(cuda):
     cache, _, _ = filled_cache([10, 20], kv_heads=2, dim=64, page=16)
     q = _q(2, 4, 64, BF16)
@@ -361,6 +379,8 @@ def test_refusals(cuda):
         PagedCache(**kw, pool=pool[:, :, :3])
     with pytest.raises(ValueError, match="contiguous"):
         PagedCache(**kw, pool=torch.zeros(1, 2, 4, 2, 32, 64, dtype=BF16, device="cuda")[:, :, :, :, :16])
+    with pytest.raises(ValueError, match="on cuda:1"):
+        PagedCache(**kw, pool=pool, device="cuda:1")
     with pytest.raises(ValueError, match="state must be"):
         PagedCache(**kw, pool=pool, state=torch.zeros(3, dtype=torch.int32, device="cuda"))
     torch.cuda.synchronize()

@@ -170,6 +170,57 @@ def test_non_finite_logits_raise(cuda):
 
 
 @pytest.mark.gpu
+def test_sliding_window_is_refused(cuda):
+    model = _tiny(F32, cuda, "qwen3")
+    for layer in model.model.layers:
+        layer.self_attn.sliding_window = 8
+    with pytest.raises(ValueError, match="sliding-window"):
+        generate(model, torch.zeros(1, 4, dtype=torch.long, device=cuda), 2, paged=True)
+    assert model.config._attn_implementation == "sdpa"
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_can_be_captured(cuda):
+    """The operators' first use on a device, inside a graph capture."""
+    import subprocess
+    import sys
+
+    from conftest import REPO
+
+    code = """
+import torch
+from s_salaad_b200.kvcache import PagedCache
+from s_salaad_b200.ops import token_logprobs
+cache = PagedCache(num_layers=1, num_pages=40, kv_heads=2, head_dim=64, max_seqs=3, max_pages=10)
+long = PagedCache(num_layers=1, num_pages=40, kv_heads=2, head_dim=64, max_seqs=3, max_pages=5000)
+k, q = torch.ones(3, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(3, 4, 64, dtype=torch.bfloat16, device="cuda")
+x, t = torch.zeros(3, 1000, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+n = torch.tensor([1, 0, 17], dtype=torch.int32, device="cuda")
+outs = []
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    for c in (cache, long):
+        c.advance(n)
+        c.append(0, k, k)
+        outs.append(c.attend(0, q))
+        c.compact()
+    outs.append(token_logprobs(x, t, top=3))
+for _ in range(3):
+    g.replay()
+torch.cuda.synchronize()
+for c in (cache, long):
+    assert c.lens.tolist() == [3, 0, 51], c.lens
+    c.check()
+assert not outs[0][1].any() and not outs[1][1].any()
+assert outs[2].top_ids.tolist() == [[0, 1, 2]] * 3
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_cache_resize_keeps_the_rows(cuda):
     model = _tiny(F32, cuda)
     cache = cache_for_model(model, 4, 100)
