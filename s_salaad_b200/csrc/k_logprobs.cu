@@ -423,14 +423,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
         sh.tau_value ? static_cast<Key>(sh.tau_value) << 32 | min(sh.tau_index[0], sh.tau_index[1]) : 0ull;
     const float tau_x = tau ? value_of(tau) : -INFINITY;
     const int groups = (n_batch + (1 << group_log) - 1) >> group_log;
-    {
-      unsigned long long mask = 0;
-      for (int g = 0; g < groups; ++g)
-        if (to_f(sh.group[g][tid]) >= tau_x) mask |= 1ull << g;
-      int at = warp_reserve(__popcll(mask), &sh.n_elig);
-      for (; mask; mask &= mask - 1, ++at)
-        if (at < kEligible) sh.elig[at] = static_cast<unsigned short>((__ffsll(mask) - 1) * kThreads + tid);
-    }
+#pragma unroll 4
+    for (int g = 0; g < groups; ++g)
+      if (to_f(sh.group[g][tid]) >= tau_x) {  // about k of all threads' groups
+        const int at = atomicAdd(&sh.n_elig, 1);
+        if (at < kEligible) sh.elig[at] = static_cast<unsigned short>(g * kThreads + tid);
+      }
     __syncthreads();
     // whether an element is a candidate (NaN counts as -inf)
     auto passes = [&](float x, int i) {

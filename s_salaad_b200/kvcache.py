@@ -11,9 +11,10 @@ lengths may differ from replay to replay).  One decode step is
   :meth:`PagedCache.attend` (one query token per row).
 
 Calls on one cache belong on one stream at a time, in order (as for any tensor
-that they update); scratch memory comes from torch's allocator per call, so
-caches, streams and graphs never share it.  The reference keeps no cache
-(``ssalaad/inference/generate.py:12-26`` recomputes the prefix).
+that they update), but :meth:`PagedCache.attend` may run on several: it only
+reads the cache, and its scratch memory comes from torch's allocator per call.
+The reference keeps no cache (``ssalaad/inference/generate.py:12-26``
+recomputes the prefix).
 """
 from __future__ import annotations
 
@@ -111,6 +112,8 @@ class PagedCache:
         self._pages_ws = int(lib.slr_kv_pages_workspace_size(self._ref))
         if not self._pages_ws:
             raise ValueError(f"PagedCache: {_lib.last_error()}")
+        # Scratch of the book-keeping: its calls change the state, so they are in order anyway.
+        self._ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=device)
         self._attend_ws: dict = {}
         self._index = device.index  # calls compare this number: cheaper than torch.device
 
@@ -162,9 +165,8 @@ class PagedCache:
             parents = self._vector("parents", parents, self.max_seqs)
         back = _switch(self._index)
         try:
-            ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=self.device)
             rc = self._lib.slr_kv_advance(self._ref, None if parents is None else parents.data_ptr(), n_ptr, n_all,
-                                          ws.data_ptr(), self._pages_ws, _stream(self.device))
+                                          self._ws.data_ptr(), self._pages_ws, _stream(self.device))
         finally:
             if back >= 0:
                 torch.cuda.set_device(back)
@@ -177,8 +179,7 @@ class PagedCache:
         free then."""
         back = _switch(self._index)
         try:
-            ws = torch.empty(self._pages_ws, dtype=torch.uint8, device=self.device)
-            rc = self._lib.slr_kv_compact(self._ref, ws.data_ptr(), self._pages_ws, _stream(self.device))
+            rc = self._lib.slr_kv_compact(self._ref, self._ws.data_ptr(), self._pages_ws, _stream(self.device))
         finally:
             if back >= 0:
                 torch.cuda.set_device(back)
