@@ -230,6 +230,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
   const int64_t r = blockIdx.x / parts;
+  pdl_wait_primary();
+  pdl_launch_dependents();
   const Row<T> row(static_cast<const T*>(a.logits) + r * a.row_stride, int(a.vocab));
   const int per = (row.vectors + parts - 1) / parts;
   const int v0 = min(row.vectors, part * per), v1 = min(row.vectors, v0 + per);
@@ -571,7 +573,9 @@ template <typename T> int launch(const LogprobArgs& a, cudaStream_t s) {
   SLR_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   int parts = 1;
   while (parts < 8 && a.rows * parts < 4 * sms && a.vocab / Vec<T>::E >= int64_t(2) * parts * kThreads) parts *= 2;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // waits for the kernel before it first
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = unsigned(parts);
   attr[0].val.clusterDim.y = 1;
@@ -581,7 +585,7 @@ template <typename T> int launch(const LogprobArgs& a, cudaStream_t s) {
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a));
   return SLR_OK;
 }
