@@ -5,7 +5,7 @@
 //
 // Bound by reading the logits once (16-bit types: the exp2 rate, 16 per clock
 // and SM, is close behind).  Each thread streams 16-byte vectors and keeps a
-// running maximum m and the sums s = Σ 2^t and u = Σ t 2^t with
+// running reference m near the maximum and the sums s = Σ 2^t and u = Σ t 2^t with
 // t = (x - m)·log2 e; the triples join associatively: over a thread's batches,
 // a block and a cluster of CTAs that share a row (few rows: up to 8 CTAs per
 // row through distributed shared memory, one launch, no workspace; many rows:
@@ -73,7 +73,7 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
 }
 
 struct Sums {
-  float m, s, u;  // m = -inf: nothing but -inf (s = 0) or NaN so far
+  float m, s, u;  // m: the reference of s and u; -inf: nothing but -inf (s = 0) or NaN so far
 };
 // (a - b) log2 e, finite: a product with a sum of 0 stays 0.  The difference
 // is taken first: logits of the type's lowest value times log2 e overflow.
@@ -151,6 +151,7 @@ template <> struct Vec<float> {
   }
   __device__ static Top greater(Top a, Top b) { return fmaxf(a, b); }
   __device__ static float of_top(Top a) { return a; }
+  __device__ static Top none() { return -INFINITY; }
 };
 template <typename T, typename P> struct Vec16 {
   static constexpr int E = 8;
@@ -182,6 +183,7 @@ template <typename T, typename P> struct Vec16 {
   }
   __device__ static Top greater(Top a, Top b) { return __hmax2(a, b); }
   __device__ static float of_top(Top a) { return fmaxf(to_f(a.x), to_f(a.y)); }
+  __device__ static Top none() { return {from_f<T>(-INFINITY), from_f<T>(-INFINITY)}; }
 };
 template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
   static constexpr float kClip = -1e38f, kLow = -1e37f, kHigh = 1e37f;
@@ -241,13 +243,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
 
   // ---- one pass: sums, and each thread's greatest value with the elements it was found among
   Sums st = {-INFINITY, 0.f, 0.f};
+  int j = v0 + tid;
   float best = -INFINITY;
-  int best_last = -1;  // index of the last element of the vector that held it
+  int best_j = j;                // the batch that held it, and its vectors' greatest
+  typename V::Top best_top[kBatch];
+#pragma unroll
+  for (int b = 0; b < kBatch; ++b) best_top[b] = V::none();
   const int batches = max(1, (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch));
   const int group_log = 32 - __clz((batches + kGroups<T> - 1) / kGroups<T> * 2 - 1) - 1;  // batches: a power of two
   int n_batch = 0;
   float in_group = -INFINITY;
-  auto raise = [&](float to) {  // the running maximum
+  auto raise = [&](float to) {
     const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, to), f = st.m == -INFINITY ? 0.f : ex2(d);
     st.u = f * (st.u + st.s * d);
     st.s *= f;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   };
   // log2 e times the maximum; 0 (every 2^t is 0 then) until there is one that the product holds
   auto base = [&] { return st.m > V::kLow ? st.m * kLog2e : 0.f; };
-  auto batch = [&](const uint4* v, const int j, const int n) {
+  auto batch = [&](const uint4* v, const int j) {
     typename V::Top top[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) top[b] = V::top(v[b]);
@@ -263,20 +269,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
 #pragma unroll
     for (int b = 1; b < kBatch; ++b) all = V::greater(all, top[b]);
     const float most = V::of_top(all);
-    if (most > st.m) raise(most);
+    // m follows the maximum within 8 (2^t up to 3000): a new greatest value of
+    // one lane, which most batches have, then rarely costs the warp a rescaling
+    if (most > st.m + 8.f) raise(most);
     if (a.top) {
       in_group = (n_batch & ((1 << group_log) - 1)) ? fmaxf(in_group, most) : most;
       sh.group[n_batch++ >> group_log][tid] = from_f<T>(in_group);  // exact
-    }
-    if (most > best || best_last < 0) {
+      const bool up = most > best;
+      best = up ? most : best;
+      best_j = up ? j : best_j;
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const float x = V::of_top(top[b]);
-        if (b < n && (x > best || best_last < 0)) {
-          best = x == x ? x : -INFINITY;  // all NaN
-          best_last = row.first_of(j + b * kThreads) + E - 1;
-        }
-      }
+      for (int b = 0; b < kBatch; ++b) best_top[b] = up ? top[b] : best_top[b];
     }
     const float m2 = base();
     const Pair scale2 = pair(kLog2e, kLog2e), base2 = pair(-m2, -m2);
@@ -301,7 +304,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
     st.s += s0 + s1;
     st.u += u0 + u1;
   };
-  int j = v0 + tid;
   constexpr int kSpan = kBatch * kThreads;
   auto whole = [&](int at) { return at + kSpan - kThreads < v1; };
   auto fetch = [&](uint4* v, int at) {
@@ -314,36 +316,43 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
     fetch(v, j);
     while (true) {
       if (!whole(j + kSpan)) {
-        batch(v, j, kBatch);
+        batch(v, j);
         j += kSpan;
         break;
       }
       fetch(next, j + kSpan);
-      batch(v, j, kBatch);
+      batch(v, j);
       j += kSpan;
       if (!whole(j + kSpan)) {
-        batch(next, j, kBatch);
+        batch(next, j);
         j += kSpan;
         break;
       }
       fetch(v, j + kSpan);
-      batch(next, j, kBatch);
+      batch(next, j);
       j += kSpan;
     }
   }
   if (j < v1) {
     uint4 v[kBatch];
-    const T none = from_f<T>(-INFINITY);
-    uint32_t word;
-    if constexpr (sizeof(T) == 4) word = __float_as_uint(-INFINITY);
-    else word = uint32_t(*reinterpret_cast<const unsigned short*>(&none)) * 0x10001u;
+    const typename V::Top none = V::none();
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(&none);
     const int n = (v1 - j + kThreads - 1) / kThreads;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) v[b] = b < n ? row.load(j + b * kThreads) : make_uint4(word, word, word, word);
-    batch(v, j, n);
+    batch(v, j);
+  }
+  // index of the last element of the vector that held the greatest value; -1: no element
+  int best_last = -1;
+  if (v0 + tid < v1) {
+    int b = 0;
+#pragma unroll
+    for (int i = kBatch - 1; i >= 0; --i)
+      if (V::of_top(best_top[i]) == best) b = best == -INFINITY ? 0 : i;
+    best_last = row.first_of(best_j + b * kThreads) + E - 1;
   }
   if (edge) {
-    if (edge_x > st.m) raise(edge_x);
+    if (edge_x > st.m + 8.f) raise(edge_x);
     const float x = edge_x < V::kClip ? V::kClip : edge_x;
     const float t = fmaf(x, kLog2e, -base()), p = ex2(t);
     st.s += p;
