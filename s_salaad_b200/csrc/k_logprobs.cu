@@ -205,7 +205,8 @@ template <typename T> struct Row {
     vectors = (vocab - head) / E;
     edges = vocab - vectors * E;
   }
-  __device__ uint4 load(int j) const { return __ldg(reinterpret_cast<const uint4*>(x + head) + j); }
+  __device__ const uint4* at(int j) const { return reinterpret_cast<const uint4*>(x + head) + j; }
+  __device__ uint4 load(int j) const { return __ldg(at(j)); }
   __device__ int first_of(int j) const { return head + j * E; }
   // element index of edge e < edges
   __device__ int edge(int e) const { return e < head ? e : e + vectors * E; }
@@ -243,15 +244,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
 
   // ---- one pass: sums, and each thread's greatest value with the elements it was found among
   Sums st = {-INFINITY, 0.f, 0.f};
-  int j = v0 + tid;
   float best = -INFINITY;
-  int best_j = j;                // the batch that held it, and its vectors' greatest
-  typename V::Top best_top[kBatch];
+  // where it was: the batch, and of 16-bit types its vectors' greatest (fp32: the vector at once)
+  constexpr bool kLate = sizeof(T) == 2;
+  int best_at = 0;
+  typename V::Top best_top[kLate ? kBatch : 1];
 #pragma unroll
-  for (int b = 0; b < kBatch; ++b) best_top[b] = V::none();
+  for (int b = 0; b < (kLate ? kBatch : 1); ++b) best_top[b] = V::none();
   const int batches = max(1, (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch));
   const int group_log = 32 - __clz((batches + kGroups<T> - 1) / kGroups<T> * 2 - 1) - 1;  // batches: a power of two
-  int n_batch = 0;
   float in_group = -INFINITY;
   auto raise = [&](float to) {
     const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, to), f = st.m == -INFINITY ? 0.f : ex2(d);
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   };
   // log2 e times the maximum; 0 (every 2^t is 0 then) until there is one that the product holds
   auto base = [&] { return st.m > V::kLow ? st.m * kLog2e : 0.f; };
-  auto batch = [&](const uint4* v, const int j) {
+  auto batch = [&](const uint4* v, const int it) {
     typename V::Top top[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) top[b] = V::top(v[b]);
@@ -273,13 +274,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
     // one lane, which most batches have, then rarely costs the warp a rescaling
     if (most > st.m + 8.f) raise(most);
     if (a.top) {
-      in_group = (n_batch & ((1 << group_log) - 1)) ? fmaxf(in_group, most) : most;
-      sh.group[n_batch++ >> group_log][tid] = from_f<T>(in_group);  // exact
+      in_group = (it & ((1 << group_log) - 1)) ? fmaxf(in_group, most) : most;
+      sh.group[it >> group_log][tid] = from_f<T>(in_group);  // exact
       const bool up = most > best;
       best = up ? most : best;
-      best_j = up ? j : best_j;
+      int at = it * kBatch;
+      if constexpr (kLate) {
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) best_top[b] = up ? top[b] : best_top[b];
+        for (int b = 0; b < kBatch; ++b) best_top[b] = up ? top[b] : best_top[b];
+      } else {
+        at += V::of_top(top[0]) == most ? 0 : V::of_top(top[1]) == most ? 1 : V::of_top(top[2]) == most ? 2 : 3;
+      }
+      best_at = up ? at : best_at;
     }
     const float m2 = base();
     const Pair scale2 = pair(kLog2e, kLog2e), base2 = pair(-m2, -m2);
@@ -305,51 +311,49 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
     st.u += u0 + u1;
   };
   constexpr int kSpan = kBatch * kThreads;
-  auto whole = [&](int at) { return at + kSpan - kThreads < v1; };
-  auto fetch = [&](uint4* v, int at) {
+  const int mine = v1 - v0 > tid ? (v1 - v0 - tid + kThreads - 1) / kThreads : 0;  // vectors of this thread
+  const int n_whole = mine / kBatch, n_batch = (mine + kBatch - 1) / kBatch;
+  const uint4* src = row.at(v0 + tid);
+  auto fetch = [&](uint4* v) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = row.load(at + b * kThreads);
+    for (int b = 0; b < kBatch; ++b) v[b] = __ldg(src + b * kThreads);
+    src += kSpan;
   };
   // the next batch is under way while one is summed
-  if (whole(j)) {
+  if (n_whole) {
     uint4 v[kBatch], next[kBatch];
-    fetch(v, j);
-    while (true) {
-      if (!whole(j + kSpan)) {
-        batch(v, j);
-        j += kSpan;
-        break;
-      }
-      fetch(next, j + kSpan);
-      batch(v, j);
-      j += kSpan;
-      if (!whole(j + kSpan)) {
-        batch(next, j);
-        j += kSpan;
-        break;
-      }
-      fetch(v, j + kSpan);
-      batch(next, j);
-      j += kSpan;
+    fetch(v);
+    int it = 0;
+    for (; it + 2 < n_whole; it += 2) {
+      fetch(next);
+      batch(v, it);
+      fetch(v);
+      batch(next, it + 1);
     }
+    if (it + 1 < n_whole) fetch(next);
+    batch(v, it);
+    if (it + 1 < n_whole) batch(next, it + 1);
   }
-  if (j < v1) {
+  if (n_batch > n_whole) {
     uint4 v[kBatch];
     const typename V::Top none = V::none();
     const uint32_t word = *reinterpret_cast<const uint32_t*>(&none);
-    const int n = (v1 - j + kThreads - 1) / kThreads;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = b < n ? row.load(j + b * kThreads) : make_uint4(word, word, word, word);
-    batch(v, j);
+    for (int b = 0; b < kBatch; ++b)
+      v[b] = n_whole * kBatch + b < mine ? __ldg(src + b * kThreads) : make_uint4(word, word, word, word);
+    batch(v, n_whole);
   }
   // index of the last element of the vector that held the greatest value; -1: no element
   int best_last = -1;
-  if (v0 + tid < v1) {
-    int b = 0;
+  if (mine) {
+    if constexpr (kLate) {
+      int b = 0;
 #pragma unroll
-    for (int i = kBatch - 1; i >= 0; --i)
-      if (V::of_top(best_top[i]) == best) b = best == -INFINITY ? 0 : i;
-    best_last = row.first_of(best_j + b * kThreads) + E - 1;
+      for (int i = kBatch - 1; i >= 0; --i)
+        if (V::of_top(best_top[i]) == best) b = best == -INFINITY ? 0 : i;
+      best_at += b;
+    }
+    best_last = row.first_of(v0 + tid + best_at * kThreads) + E - 1;
   }
   if (edge) {
     if (edge_x > st.m + 8.f) raise(edge_x);
