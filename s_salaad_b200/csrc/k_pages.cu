@@ -9,6 +9,8 @@
 // per thread, over all layers' K and V at once.  Every choice is made in row
 // and page order, so the state never depends on timing; the only atomics are
 // integer sums and minima.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -59,63 +61,58 @@ __device__ __forceinline__ int checked_parent(const PagesK& p, const int32_t* pa
   return from >= p.rows || from < 0 ? -1 : from;
 }
 
-// Table rows become their parents' rows, entries behind the kept length -1.
-// Columns are independent, so a CTA reads its kCols columns of every row
-// before it writes them: in place, one launch.  refs follow by integer
-// atomics, per parent: its pages gain (children - 1) references, nothing where
-// a row merely moves, and each child loses those behind its kept length.  Each
-// CTA adds its change of the number of live pages.  Bound by latency: few
-// columns per CTA, everything read at once (250 rows x 120 pages: 32 columns
-// and two atomics per entry took 54 us, 4 columns 11).
-constexpr int kCols = 4;
-constexpr int kEarly = 4;  // entries that a thread reads before the lengths are known
-__global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32_t* parents, const int32_t* n_new,
-                                                     int n_all) {
-  extern __shared__ int32_t sm[];
-  int32_t* old = sm;                     // [rows][kCols]
-  int32_t* len = old + p.rows * kCols;   // [rows] lengths before
-  int32_t* from = len + p.rows;          // [rows]
-  int32_t* children = from + p.rows;     // [rows]
-  __shared__ int s_most, s_live;
-  const int tid = threadIdx.x, c0 = blockIdx.x * kCols;
-  pdl_wait_primary();
-  pdl_launch_dependents();
-  auto entry = [&](int i) {
-    const int c = c0 + i % kCols;
-    return c < p.max_pages ? p.table[int64_t(i / kCols) * p.max_pages + c] : -1;
-  };
-  int early[kEarly];
-#pragma unroll
-  for (int k = 0; k < kEarly; ++k) {
-    const int i = k * int(blockDim.x) + tid;
-    early[k] = i < p.rows * kCols ? entry(i) : -1;
-  }
-  if (tid == 0) s_most = 0, s_live = 0;
+// What a selection does, in shared memory.
+struct Selection {
+  int32_t* old;       // [rows][columns of a step] table entries before
+  int32_t* len;       // [rows] lengths before
+  int32_t* from;      // [rows] parents
+  int32_t* children;  // [rows]
+};
+template <int kC> __device__ __forceinline__ Selection selection_at(int32_t* sm, int rows) {
+  Selection s;
+  s.old = sm;
+  s.len = s.old + rows * kC;
+  s.from = s.len + rows;
+  s.children = s.from + rows;
+  return s;
+}
+
+// Reads lengths and parents and counts children; the greatest length in
+// *s_most (0 before).  Ends with a barrier.
+__device__ __forceinline__ void read_selection(const PagesK& p, const int32_t* parents, const Selection& s, int* s_most,
+                                               bool report) {
+  const int tid = threadIdx.x;
   bool bad = false;
   int most = 0;
   for (int r = tid; r < p.rows; r += blockDim.x) {
-    from[r] = checked_parent(p, parents, r, &bad);
-    len[r] = checked_length(p, r, &bad);
-    children[r] = 0;
-    most = max(most, len[r]);
+    s.from[r] = checked_parent(p, parents, r, &bad);
+    s.len[r] = checked_length(p, r, &bad);
+    s.children[r] = 0;
+    most = max(most, s.len[r]);
   }
   __syncthreads();
   most = __reduce_max_sync(0xffffffffu, most);
-  if ((tid & 31) == 0) atomicMax(&s_most, most);
+  if ((tid & 31) == 0) atomicMax(s_most, most);
   for (int r = tid; r < p.rows; r += blockDim.x)
-    if (from[r] >= 0) atomicAdd(children + from[r], 1);
-  if (bad && blockIdx.x == 0) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
-#pragma unroll
-  for (int k = 0; k < kEarly; ++k) {
-    const int i = k * int(blockDim.x) + tid;
-    if (i < p.rows * kCols) old[i] = early[k];
-  }
+    if (s.from[r] >= 0) atomicAdd(s.children + s.from[r], 1);
+  if (bad && report) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
   __syncthreads();
-  // no row has an entry from here on: there is nothing to move or to drop
-  if (c0 >= pages_of(s_most, p.page_size)) return;
-#pragma unroll 4
-  for (int i = kEarly * int(blockDim.x) + tid; i < p.rows * kCols; i += blockDim.x) old[i] = entry(i);
-  __syncthreads();
+}
+
+template <int kC> __device__ __forceinline__ int table_entry(const PagesK& p, int c0, int i) {
+  const int c = c0 + i % kC;
+  return c < p.max_pages ? p.table[int64_t(i / kC) * p.max_pages + c] : -1;
+}
+
+// Columns [c0, c0 + kC) of all rows, once `old` holds them: table rows become
+// their parents' rows, entries behind the kept length -1.  Columns are
+// independent, so this works in place.  refs follow by integer atomics, per
+// parent: its pages gain (children - 1) references, nothing where a row merely
+// moves, and each child loses those behind its kept length.  Returns this
+// thread's change of the number of live pages.
+template <int kC>
+__device__ __forceinline__ int select_columns(const PagesK& p, const Selection& s, const int32_t* n_new, int n_all,
+                                              int c0) {
   int live = 0;
   auto refer = [&](int page, int change) {
     if (page < 0) return;
@@ -128,15 +125,15 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
     live += int(was + change > 0) - int(was > 0);
   };
 #pragma unroll 2
-  for (int i = tid; i < p.rows * kCols; i += blockDim.x) {
-    const int r = i / kCols, j = i % kCols, c = c0 + j;
+  for (int i = threadIdx.x; i < p.rows * kC; i += blockDim.x) {
+    const int r = i / kC, j = i % kC, c = c0 + j;
     if (c >= p.max_pages) continue;
-    const int was = old[i], f = from[r];
-    if (children[r] != 1) refer(was, children[r] - 1);
+    const int was = s.old[i], f = s.from[r];
+    if (s.children[r] != 1) refer(was, s.children[r] - 1);
     int now = -1;
     if (f >= 0) {
-      now = old[f * kCols + j];
-      const int keep = kept_length(len[f], n_new ? n_new[r] : n_all);
+      now = s.old[f * kC + j];
+      const int keep = kept_length(s.len[f], n_new ? n_new[r] : n_all);
       if (c >= pages_of(keep, p.page_size)) {
         refer(now, -1);
         now = -1;
@@ -144,10 +141,50 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
     }
     if (was != now) p.table[int64_t(r) * p.max_pages + c] = now;
   }
+  return live;
+}
+
+// Adds the threads' changes to the header.
+__device__ __forceinline__ void add_live(const PagesK& p, int live, int* s_live) {
   live = __reduce_add_sync(0xffffffffu, live);
-  if ((tid & 31) == 0 && live) atomicAdd(&s_live, live);
+  if ((threadIdx.x & 31) == 0 && live) atomicAdd(s_live, live);
   __syncthreads();
-  if (tid == 0 && s_live) atomicAdd(p.head + kLive, s_live);
+  if (threadIdx.x == 0 && *s_live) atomicAdd(p.head + kLive, *s_live);
+}
+
+// A selection over a large table: few columns per CTA, all read at once, since
+// latency is the bound (250 rows x 120 pages: 32 columns and two atomics per
+// entry took 54 us, 4 columns 11).
+constexpr int kCols = 4;
+constexpr int kEarly = 4;  // entries that a thread reads before the lengths are known
+__global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32_t* parents, const int32_t* n_new,
+                                                     int n_all) {
+  extern __shared__ int32_t sm[];
+  const Selection s = selection_at<kCols>(sm, p.rows);
+  __shared__ int s_most, s_live;
+  const int tid = threadIdx.x, c0 = blockIdx.x * kCols;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  int early[kEarly];
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int i = k * int(blockDim.x) + tid;
+    early[k] = i < p.rows * kCols ? table_entry<kCols>(p, c0, i) : -1;
+  }
+  if (tid == 0) s_most = 0, s_live = 0;
+  read_selection(p, parents, s, &s_most, blockIdx.x == 0);
+  // no row has an entry from here on: there is nothing to move or to drop
+  if (c0 >= pages_of(s_most, p.page_size)) return;
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int i = k * int(blockDim.x) + tid;
+    if (i < p.rows * kCols) s.old[i] = early[k];
+  }
+#pragma unroll 4
+  for (int i = kEarly * int(blockDim.x) + tid; i < p.rows * kCols; i += blockDim.x)
+    s.old[i] = table_entry<kCols>(p, c0, i);
+  __syncthreads();
+  add_live(p, select_columns<kCols>(p, s, n_new, n_all, c0), &s_live);
 }
 
 constexpr int kGrowThreads = 1024;
@@ -184,16 +221,17 @@ __device__ __forceinline__ unsigned free_mask(const PagesK& p, int64_t i0) {
   unsigned mask = 0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j)
-    if (i0 + j < p.num_pages && p.refs[i0 + j] == 0) mask |= 1u << j;
+    if (i0 + j < p.num_pages && __ldcg(p.refs + i0 + j) == 0) mask |= 1u << j;
   return mask;
 }
 
-// Growth of every row: one CTA.  Pages are given out lowest number first in
+// Growth of every row, by one CTA.  Pages are given out lowest number first in
 // row order, a row's copy of a shared last page before its new pages.  Bound
-// by the latency of its chain of reads (parents, lens, table, refs).
-__global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, const int32_t* parents,
-                                                               const int32_t* n_new, int n_all) {
-  extern __shared__ int32_t sm[];
+// by the latency of its chain of reads (lens and parents, table, refs).
+// before: the selection when it was made in this kernel, else null.  What
+// other CTAs of the cluster have written is read past L1.
+__device__ __forceinline__ void grow_rows(const PagesK& p, const int32_t* parents, const int32_t* n_new, int n_all,
+                                          int32_t* sm, const Selection* before) {
   int32_t* low = sm;              // [rows] kept lengths
   int32_t* start = low + p.rows;  // [rows + 1] pages given to the rows before
   int32_t* copy = start + p.rows + 1;
@@ -201,8 +239,6 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
   __shared__ int sums[32];
   __shared__ int s_over, s_list[kListed];
   const int tid = threadIdx.x;
-  pdl_wait_primary();
-  pdl_launch_dependents();
   const unsigned first_free = free_mask(p, int64_t(tid) * kPer);  // read early: most calls need no more
   if (tid == 0) s_over = 0;
   const int64_t cap = int64_t(p.max_pages) * p.page_size;
@@ -211,26 +247,28 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     const int64_t n = n_new ? n_new[r] : n_all;
     return n <= 0 || (!n_new && low[r] == 0) ? 0 : n;  // one number for all: rows that hold tokens
   };
-  // lens and parents are read side by side; start holds the lengths before for a moment
-  for (int r = tid; r < p.rows; r += kGrowThreads) {
-    copy[r] = checked_parent(p, parents, r, &bad);
-    start[r] = checked_length(p, r, &bad);
+  if (!before) {
+    // lens and parents are read side by side; start holds the lengths before for a moment
+    for (int r = tid; r < p.rows; r += kGrowThreads) {
+      copy[r] = checked_parent(p, parents, r, &bad);
+      start[r] = checked_length(p, r, &bad);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int r = tid; r < p.rows; r += kGrowThreads) {
-    const int from = copy[r];
-    low[r] = from < 0 ? 0 : kept_length(start[from], n_new ? n_new[r] : n_all);
-  }
+  const int32_t* from = before ? before->from : copy;
+  const int32_t* len = before ? before->len : start;
+  for (int r = tid; r < p.rows; r += kGrowThreads)
+    low[r] = from[r] < 0 ? 0 : kept_length(len[from[r]], n_new ? n_new[r] : n_all);
   __syncthreads();
   // rows about to write into a shared last page
   auto shared_last = [&](int r) -> int {
     if (grow_of(r) == 0 || low[r] % p.page_size == 0) return -1;
-    const int last = p.table[int64_t(r) * p.max_pages + low[r] / p.page_size];
+    const int last = __ldcg(p.table + int64_t(r) * p.max_pages + low[r] / p.page_size);
     if (last < 0 || last >= p.num_pages) {
       bad = true;
       return -1;
     }
-    return p.refs[last] > 1 ? last : -1;
+    return __ldcg(p.refs + last) > 1 ? last : -1;
   };
   bool any = false;
   for (int r = tid; r < p.rows; r += kGrowThreads) {
@@ -256,7 +294,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
     return pages_of(low[r] + grow_of(r), p.page_size) - pages_of(low[r], p.page_size) + (copy[r] >= 0 ? 1 : 0);
   };
   for (int r = r0; r < r1; ++r) {
-    if (copy[r] >= 0 && __ldcg(p.growers + copy[r]) == p.refs[copy[r]] && __ldcg(p.first + copy[r]) == r) copy[r] = -1;
+    if (copy[r] >= 0 && __ldcg(p.growers + copy[r]) == __ldcg(p.refs + copy[r]) && __ldcg(p.first + copy[r]) == r) copy[r] = -1;
     mine += need_of(r);
   }
   int64_t total = 0;
@@ -319,7 +357,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
       p.head[kShort] = 0;
       p.head[kOver] = 0;
       p.head[kCopies] = copies;
-      p.head[kLive] += int(total);
+      atomicAdd(p.head + kLive, int(total));
     }
   } else {
     for (int r = tid; r < p.rows; r += kGrowThreads) p.lens[r] = low[r];
@@ -329,6 +367,45 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
       p.head[kCopies] = 0;
     }
   }
+}
+
+__global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, const int32_t* parents,
+                                                               const int32_t* n_new, int n_all) {
+  extern __shared__ int32_t sm[];
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  grow_rows(p, parents, n_new, n_all, sm, nullptr);
+}
+
+// Selection and growth of a small table in one launch: a cluster of CTAs takes
+// the columns in turn, kStepCols at a time, then its first one grows the rows.
+// A decode step's calls are bound by the host: one launch less makes this call
+// 2.3 us shorter there (on the GPU it takes 0.3 to 0.8 us more than two).
+constexpr int kStepCols = 16, kStepCtas = 8;
+constexpr int kStepRows = 512, kStepPages = 512;  // at most: four steps of 8 entries per thread
+__global__ void __launch_bounds__(kGrowThreads, 1) step_kernel(const PagesK p, const int32_t* parents,
+                                                               const int32_t* n_new, int n_all) {
+  extern __shared__ int32_t sm[];
+  const Selection s = selection_at<kStepCols>(sm, p.rows);
+  __shared__ int s_most, s_live;
+  const int tid = threadIdx.x;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (tid == 0) s_most = 0, s_live = 0;
+  __syncthreads();
+  read_selection(p, parents, s, &s_most, blockIdx.x == 0);
+  int live = 0;
+  const int used = int(pages_of(s_most, p.page_size));
+  for (int c0 = blockIdx.x * kStepCols; c0 < used; c0 += kStepCtas * kStepCols) {
+#pragma unroll 4
+    for (int i = tid; i < p.rows * kStepCols; i += kGrowThreads) s.old[i] = table_entry<kStepCols>(p, c0, i);
+    __syncthreads();
+    live += select_columns<kStepCols>(p, s, n_new, n_all, c0);
+    __syncthreads();
+  }
+  add_live(p, live, &s_live);
+  cooperative_groups::this_cluster().sync();
+  if (blockIdx.x == 0) grow_rows(p, parents, n_new, n_all, s.old, &s);
 }
 
 // Plan of a compaction: one CTA.  Live pages from the live count on go to the
@@ -614,7 +691,30 @@ int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const
   int sms = 0;
   int rc = prepare_device(&sms);
   if (rc) return rc;
-  if (parents || n_new || n_all < 0) {
+  const bool select = parents || n_new || n_all < 0;
+  if (select && p.rows <= kStepRows && p.max_pages <= kStepPages) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kStepCtas;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kStepCtas);
+    cfg.blockDim = dim3(kGrowThreads);
+    cfg.dynamicSmemBytes = size_t(p.rows) * (kStepCols + 3) * 4;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SLR_CHECK_CUDA(cudaLaunchKernelEx(&cfg, step_kernel, k, parents, n_new, n_all));
+    CopyK c = {};
+    c.src = k.src;
+    c.dst = k.dst;
+    c.count = k.head + kCopies;
+    return copy_launch(p, c, p.rows, 8 * sms, s);
+  }
+  if (select) {
     const size_t smem = size_t(p.rows) * (kCols + 3) * 4;
     rc = launch_after(select_kernel, dim3(unsigned(ceil_div(p.max_pages, kCols))), 256, smem, s, k, parents,
                                 n_new, n_all);
