@@ -546,26 +546,31 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
     } else {
       // lane = token (lane & 7) x quarter of the head dimension (lane >> 3)
       const int t = lane & 7, qt = lane >> 3;
-      float s[GT] = {};
+      Pair s2[GT] = {};  // even and odd columns
       const uint8_t* stage = ring + (base - smem_u32(ring));
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         const int ch = qt * (DP / 16) + i;
-        const float4 kv = *reinterpret_cast<const float4*>(stage + t * C::kRow + ((ch ^ t) << 4));
+        const ulonglong2 kv = *reinterpret_cast<const ulonglong2*>(stage + t * C::kRow + ((ch ^ t) << 4));
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
-          float4 qv;
+          ulonglong2 qv;
           if constexpr (C::kQRegs) {
             const float* x = qr + g * (DP / 4) + i * 4;
-            qv = make_float4(x[0], x[1], x[2], x[3]);
+            qv = make_ulonglong2(pair(x[0], x[1]), pair(x[2], x[3]));
           } else {
-            qv = *reinterpret_cast<const float4*>(qs + g * DP + ch * 4);
+            qv = *reinterpret_cast<const ulonglong2*>(qs + g * DP + ch * 4);
           }
-          s[g] = fmaf(qv.x, kv.x, s[g]);
-          s[g] = fmaf(qv.y, kv.y, s[g]);
-          s[g] = fmaf(qv.z, kv.z, s[g]);
-          s[g] = fmaf(qv.w, kv.w, s[g]);
+          s2[g] = fma2(qv.x, kv.x, s2[g]);
+          s2[g] = fma2(qv.y, kv.y, s2[g]);
         }
+      }
+      float s[GT];
+#pragma unroll
+      for (int g = 0; g < GT; ++g) {
+        float even, odd;
+        unpair(s2[g], even, odd);
+        s[g] = even + odd;
       }
       float* pw = ps + w * TT * GT;
 #pragma unroll
@@ -592,15 +597,15 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       __syncwarp();
       const uint8_t* vr = stage + C::kHalf;
       auto add = [&](int tt) {
-        float vv[DP / 32], pg[GT];
+        Pair vv[DP / 64];
+        float pg[GT];
         if constexpr (DP == 64) {
-          const float2 x = *reinterpret_cast<const float2*>(vr + tt * C::kRow + (((lane >> 1) ^ tt) << 4) + (lane & 1) * 8);
-          vv[0] = x.x, vv[1] = x.y;
+          vv[0] = *reinterpret_cast<const Pair*>(vr + tt * C::kRow + (((lane >> 1) ^ tt) << 4) + (lane & 1) * 8);
         } else {
 #pragma unroll
           for (int j = 0; j < DP / 128; ++j) {
-            const float4 x = *reinterpret_cast<const float4*>(vr + tt * C::kRow + (((j * 32 + lane) ^ tt) << 4));
-            vv[j * 4] = x.x, vv[j * 4 + 1] = x.y, vv[j * 4 + 2] = x.z, vv[j * 4 + 3] = x.w;
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(vr + tt * C::kRow + (((j * 32 + lane) ^ tt) << 4));
+            vv[j * 2] = x.x, vv[j * 2 + 1] = x.y;
           }
         }
         if constexpr (GT % 4 == 0) {
@@ -614,9 +619,14 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
           for (int g = 0; g < GT; ++g) pg[g] = pw[tt * GT + g];
         }
 #pragma unroll
-        for (int g = 0; g < GT; ++g)
+        for (int g = 0; g < GT; ++g) {
+          const Pair p2 = pair(pg[g], pg[g]);
 #pragma unroll
-          for (int i = 0; i < DP / 32; ++i) o[g * (DP / 32) + i] = fmaf(pg[g], vv[i], o[g * (DP / 32) + i]);
+          for (int i = 0; i < DP / 64; ++i) {
+            float* at = o + g * (DP / 32) + i * 2;
+            unpair(fma2(p2, vv[i], pair(at[0], at[1])), at[0], at[1]);
+          }
+        }
       };
       // rows behind the length are zeros in the stage, their p is 0
 #pragma unroll

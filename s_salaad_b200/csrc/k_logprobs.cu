@@ -57,25 +57,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Two fp32 in one 64-bit register pair: one instruction for both.
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(Pair p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 struct Sums {
   float m, s, u;  // m: the reference of s and u; -inf: nothing but -inf (s = 0) or NaN so far
 };
