@@ -51,6 +51,11 @@ constexpr int kMinTiles = 2;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// The reference of the exponentials follows the running maximum within this
+// many powers of two: most tiles then need one vote instead of a maximum over
+// the lanes and a rescaling.
+constexpr float kSlack = 8.f;
+
 struct AttendK {
   const void* k;
   const void* v;
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) load_stage();
 
-  // ---- running softmax of this warp: log2-domain maximum, sum, output
+  // ---- running softmax of this warp: log2-domain reference, sum, output
   // 16-bit: the MMAs compute Sᵀ = K · Qᵀ (16 tokens x 8 heads) and Oᵀ = Vᵀ · Pᵀ
   // (16 columns x 8 heads), so a lane has heads 2 (lane % 4) and + 1 of every
   // 8 in both; groups of up to 8 heads waste no MMA on empty rows.
@@ -474,13 +479,13 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
             mma16816<T>::run(s[nt][ks & 1], k, qf[(ks * NT + nt) * 2], qf[(ks * NT + nt) * 2 + 1]);
         }
       }
+      // With scale < 0 the largest product is the smallest score: the maximum is taken after scaling.
       float mn[kStat];
       bool grew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[nt][0][e] += s[nt][1][e];
-        // With scale < 0 the largest product is the smallest score: the maximum is taken after scaling.
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float x0 = s[nt][0][e] * a.scale_log2, x1 = s[nt][0][e + 2] * a.scale_log2;
@@ -488,12 +493,8 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
             if ((lane >> 2) >= valid) x0 = -INFINITY;
             if ((lane >> 2) + 8 >= valid) x1 = -INFINITY;
           }
-          float x = fmaxf(x0, x1);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          mn[nt * 2 + e] = fmaxf(m[nt * 2 + e], x);
-          grew |= mn[nt * 2 + e] > m[nt * 2 + e];
+          mn[nt * 2 + e] = fmaxf(x0, x1);
+          grew |= mn[nt * 2 + e] > m[nt * 2 + e] + kSlack;
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
@@ -503,9 +504,13 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int i = nt * 2 + e;
-            fac[e] = mn[i] == m[i] ? 1.f : ex2(m[i] - mn[i]);
+            float x = fmaxf(m[i], mn[i]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            fac[e] = x == m[i] ? 1.f : ex2(m[i] - x);
             l[i] *= fac[e];
-            m[i] = mn[i];
+            m[i] = x;
           }
 #pragma unroll
           for (int i = 0; i < DP / 4; ++i) o[nt * (DP / 4) + i] *= fac[i & 1];
@@ -573,21 +578,29 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
         s[g] = even + odd;
       }
       float* pw = ps + w * TT * GT;
+      bool grew = false;
 #pragma unroll
       for (int g = 0; g < GT; ++g) {
         s[g] += __shfl_xor_sync(0xffffffffu, s[g], 8);
         s[g] += __shfl_xor_sync(0xffffffffu, s[g], 16);
-        float x = t < valid ? s[g] * a.scale_log2 : -INFINITY;
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        if (x > m[g]) {  // the same for all lanes
-          const float fac = ex2(m[g] - x);
+        grew |= t < valid && s[g] * a.scale_log2 > m[g] + kSlack;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+          float x = t < valid ? fmaxf(m[g], s[g] * a.scale_log2) : m[g];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          const float fac = x == m[g] ? 1.f : ex2(m[g] - x);
           l[g] *= fac;
 #pragma unroll
           for (int i = 0; i < DP / 32; ++i) o[g * (DP / 32) + i] *= fac;
           m[g] = x;
         }
+      }
+#pragma unroll
+      for (int g = 0; g < GT; ++g) {
         const float p = t < valid ? ex2(fmaf(s[g], a.scale_log2, m[g] == -INFINITY ? 0.f : -m[g])) : 0.f;
         if (qt == 0) {
           l[g] += p;
