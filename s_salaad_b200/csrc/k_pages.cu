@@ -67,20 +67,23 @@ struct Selection {
   int32_t* len;       // [rows] lengths before
   int32_t* from;      // [rows] parents
   int32_t* children;  // [rows]
+  int32_t* keep;      // [rows] entries of the parent that stay
 };
+constexpr int kSelectionWords = 4;  // words per row besides `old`
 template <int kC> __device__ __forceinline__ Selection selection_at(int32_t* sm, int rows) {
   Selection s;
   s.old = sm;
   s.len = s.old + rows * kC;
   s.from = s.len + rows;
   s.children = s.from + rows;
+  s.keep = s.children + rows;
   return s;
 }
 
 // Reads lengths and parents and counts children; the greatest length in
 // *s_most (0 before).  Ends with a barrier.
-__device__ __forceinline__ void read_selection(const PagesK& p, const int32_t* parents, const Selection& s, int* s_most,
-                                               bool report) {
+__device__ __forceinline__ void read_selection(const PagesK& p, const int32_t* parents, const int32_t* n_new, int n_all,
+                                               const Selection& s, int* s_most, bool report) {
   const int tid = threadIdx.x;
   bool bad = false;
   int most = 0;
@@ -88,13 +91,17 @@ __device__ __forceinline__ void read_selection(const PagesK& p, const int32_t* p
     s.from[r] = checked_parent(p, parents, r, &bad);
     s.len[r] = checked_length(p, r, &bad);
     s.children[r] = 0;
+    s.keep[r] = n_new ? n_new[r] : n_all;  // the change of length, for a moment
     most = max(most, s.len[r]);
   }
   __syncthreads();
   most = __reduce_max_sync(0xffffffffu, most);
   if ((tid & 31) == 0) atomicMax(s_most, most);
-  for (int r = tid; r < p.rows; r += blockDim.x)
-    if (s.from[r] >= 0) atomicAdd(s.children + s.from[r], 1);
+  for (int r = tid; r < p.rows; r += blockDim.x) {
+    const int f = s.from[r];
+    if (f >= 0) atomicAdd(s.children + f, 1);
+    s.keep[r] = f < 0 ? 0 : int(pages_of(kept_length(s.len[f], s.keep[r]), p.page_size));
+  }
   if (bad && report) atomicOr(&g_status_pages, SLR_BAD_INDEX_BIT);
   __syncthreads();
 }
@@ -111,8 +118,7 @@ template <int kC> __device__ __forceinline__ int table_entry(const PagesK& p, in
 // moves, and each child loses those behind its kept length.  Returns this
 // thread's change of the number of live pages.
 template <int kC>
-__device__ __forceinline__ int select_columns(const PagesK& p, const Selection& s, const int32_t* n_new, int n_all,
-                                              int c0) {
+__device__ __forceinline__ int select_columns(const PagesK& p, const Selection& s, int c0) {
   int live = 0;
   auto refer = [&](int page, int change) {
     if (page < 0) return;
@@ -124,7 +130,7 @@ __device__ __forceinline__ int select_columns(const PagesK& p, const Selection& 
     const int was = atomicAdd(p.refs + page, change);
     live += int(was + change > 0) - int(was > 0);
   };
-#pragma unroll 2
+#pragma unroll 4
   for (int i = threadIdx.x; i < p.rows * kC; i += blockDim.x) {
     const int r = i / kC, j = i % kC, c = c0 + j;
     if (c >= p.max_pages) continue;
@@ -133,8 +139,7 @@ __device__ __forceinline__ int select_columns(const PagesK& p, const Selection& 
     int now = -1;
     if (f >= 0) {
       now = s.old[f * kC + j];
-      const int keep = kept_length(s.len[f], n_new ? n_new[r] : n_all);
-      if (c >= pages_of(keep, p.page_size)) {
+      if (c >= s.keep[r]) {
         refer(now, -1);
         now = -1;
       }
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
     early[k] = i < p.rows * kCols ? table_entry<kCols>(p, c0, i) : -1;
   }
   if (tid == 0) s_most = 0, s_live = 0;
-  read_selection(p, parents, s, &s_most, blockIdx.x == 0);
+  read_selection(p, parents, n_new, n_all, s, &s_most, blockIdx.x == 0);
   // no row has an entry from here on: there is nothing to move or to drop
   if (c0 >= pages_of(s_most, p.page_size)) return;
 #pragma unroll
@@ -184,7 +189,7 @@ __global__ void __launch_bounds__(256) select_kernel(const PagesK p, const int32
   for (int i = kEarly * int(blockDim.x) + tid; i < p.rows * kCols; i += blockDim.x)
     s.old[i] = table_entry<kCols>(p, c0, i);
   __syncthreads();
-  add_live(p, select_columns<kCols>(p, s, n_new, n_all, c0), &s_live);
+  add_live(p, select_columns<kCols>(p, s, c0), &s_live);
 }
 
 constexpr int kGrowThreads = 1024;
@@ -380,7 +385,7 @@ __global__ void __launch_bounds__(kGrowThreads, 1) grow_kernel(const PagesK p, c
 // Selection and growth of a small table in one launch: a cluster of CTAs takes
 // the columns in turn, kStepCols at a time, then its first one grows the rows.
 // A decode step's calls are bound by the host: one launch less makes this call
-// 2.3 us shorter there (on the GPU it takes 0.3 to 0.8 us more than two).
+// 2.3 us shorter there (on the GPU both take the same).
 constexpr int kStepCols = 16, kStepCtas = 8;
 constexpr int kStepRows = 512, kStepPages = 512;  // at most: four steps of 8 entries per thread
 __global__ void __launch_bounds__(kGrowThreads, 1) step_kernel(const PagesK p, const int32_t* parents,
@@ -391,16 +396,31 @@ __global__ void __launch_bounds__(kGrowThreads, 1) step_kernel(const PagesK p, c
   const int tid = threadIdx.x;
   pdl_wait_primary();
   pdl_launch_dependents();
+  int early[kEarly];  // of this CTA's first columns, read beside the lengths
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int i = k * kGrowThreads + tid;
+    early[k] = i < p.rows * kStepCols ? table_entry<kStepCols>(p, blockIdx.x * kStepCols, i) : -1;
+  }
   if (tid == 0) s_most = 0, s_live = 0;
   __syncthreads();
-  read_selection(p, parents, s, &s_most, blockIdx.x == 0);
+  read_selection(p, parents, n_new, n_all, s, &s_most, blockIdx.x == 0);
   int live = 0;
   const int used = int(pages_of(s_most, p.page_size));
   for (int c0 = blockIdx.x * kStepCols; c0 < used; c0 += kStepCtas * kStepCols) {
+    int done = 0;
+    if (c0 == int(blockIdx.x) * kStepCols) {
+#pragma unroll
+      for (int k = 0; k < kEarly; ++k) {
+        const int i = k * kGrowThreads + tid;
+        if (i < p.rows * kStepCols) s.old[i] = early[k];
+      }
+      done = kEarly * kGrowThreads;
+    }
 #pragma unroll 4
-    for (int i = tid; i < p.rows * kStepCols; i += kGrowThreads) s.old[i] = table_entry<kStepCols>(p, c0, i);
+    for (int i = done + tid; i < p.rows * kStepCols; i += kGrowThreads) s.old[i] = table_entry<kStepCols>(p, c0, i);
     __syncthreads();
-    live += select_columns<kStepCols>(p, s, n_new, n_all, c0);
+    live += select_columns<kStepCols>(p, s, c0);
     __syncthreads();
   }
   add_live(p, live, &s_live);
@@ -639,7 +659,9 @@ int prepare_device(int* sms) {
   int n = dev < kDevices ? known[dev].load(std::memory_order_acquire) : 0;
   if (!n) {
     SLR_CHECK_CUDA(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        kAttendMaxRows * (kCols + 3) * 4));
+                                        kAttendMaxRows * (kCols + kSelectionWords) * 4));
+    SLR_CHECK_CUDA(cudaFuncSetAttribute(step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kStepRows * (kStepCols + kSelectionWords) * 4));
     SLR_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
     if (dev < kDevices) known[dev].store(n, std::memory_order_release);
   }
@@ -703,7 +725,7 @@ int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kStepCtas);
     cfg.blockDim = dim3(kGrowThreads);
-    cfg.dynamicSmemBytes = size_t(p.rows) * (kStepCols + 3) * 4;
+    cfg.dynamicSmemBytes = size_t(p.rows) * (kStepCols + kSelectionWords) * 4;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -715,7 +737,7 @@ int launch_kv_advance(const PagesArgs& p, const int32_t* n_new, int n_all, const
     return copy_launch(p, c, p.rows, 8 * sms, s);
   }
   if (select) {
-    const size_t smem = size_t(p.rows) * (kCols + 3) * 4;
+    const size_t smem = size_t(p.rows) * (kCols + kSelectionWords) * 4;
     rc = launch_after(select_kernel, dim3(unsigned(ceil_div(p.max_pages, kCols))), 256, smem, s, k, parents,
                                 n_new, n_all);
     if (rc) return rc;

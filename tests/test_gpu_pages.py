@@ -80,7 +80,9 @@ def test_growth_is_all_or_nothing(cuda):
     cache.check()
 
 
-@pytest.mark.parametrize("rows,pages,width", [(1, 3, 2), (7, 40, 6), (33, 300, 9), (200, 9000, 70), (700, 5000, 12)])
+@pytest.mark.parametrize("rows,pages,width", [(1, 3, 2), (7, 40, 6), (33, 300, 9), (200, 9000, 70),
+                                              (512, 6000, 512), (513, 6000, 20), (40, 3000, 513),
+                                              (700, 5000, 12)])
 def test_random_steps(cuda, rows, pages, width):
     """Random forks, ends, rollbacks, growth and compactions."""
     rng = random.Random(rows)
