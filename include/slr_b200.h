@@ -519,7 +519,10 @@ SLR_API int slr_kv_append(const slr_kv_cache* cache, int32_t layer, const void* 
  * score gives NaN.  Slots behind a row's length are never read into the
  * result, whatever they hold.  Products and sums are fp32; the
  * probabilities are kept to at least 16 bits; out is rounded once.  The
- * result does not depend on timing, only on lens and the GPU's SM count.
+ * result does not depend on timing, only on the inputs, the sizes of the call
+ * and of the cache, and the GPU's SM count.  workspace may be NULL where
+ * slr_kv_attend_workspace_size gives 0 (few rows with short tables).  out may be
+ * q itself; strides that put two of its vectors over one another are refused.  The cache is only read: calls on several streams may overlap.
  */
 SLR_API int slr_kv_attend(const slr_kv_cache* cache, int32_t layer, const void* q, int64_t q_row_stride,
                           int64_t q_head_stride, void* out, int64_t o_row_stride, int64_t o_head_stride,

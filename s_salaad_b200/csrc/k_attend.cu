@@ -991,9 +991,9 @@ struct Inst {
     a.part_o = reinterpret_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + size_t(2 * a.workers) * C::GT * DP * 4);
     a.prefix = reinterpret_cast<int32_t*>(ws + size_t(2 * a.workers) * C::GT * (DP * 4 + 8));
-    if (!small && need(a.workers, a.rows) > x.workspace_bytes)
+    if (!small && (!ws || need(a.workers, a.rows) > x.workspace_bytes))
       return fail(SLR_ERR_WORKSPACE,
-                  "attend: workspace too small, need " + std::to_string(need(a.workers, a.rows)) + " bytes");
+                  "attend: workspace is NULL or too small, need " + std::to_string(need(a.workers, a.rows)) + " bytes");
     cudaLaunchAttribute attr[2];
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = unsigned(std::max(small, 1));

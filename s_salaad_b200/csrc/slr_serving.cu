@@ -179,6 +179,14 @@ int slr_kv_attend(const slr_kv_cache* cache, int32_t layer, const void* q, int64
   if (rows == 0) return SLR_OK;
   if (!q || !out) return fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: q or out is NULL");
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(SLR_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  // every output vector has its own place: the heads within a row's stride, or the rows within a head's
+  auto apart = [&](int64_t n_in, int64_t in, int64_t n_out, int64_t outer) {
+    if (n_in > 1 && in < cache->head_dim) return false;
+    const __int128 span = (n_in > 1 ? __int128(in) * (n_in - 1) : 0) + cache->head_dim;
+    return n_out <= 1 || outer >= span;
+  };
+  if (!apart(heads, o_head_stride, rows, o_row_stride) && !apart(rows, o_row_stride, heads, o_head_stride))
+    return fail(SLR_ERR_INVALID_ARGUMENT, "kv attend: out overlaps itself");
   AttendArgs a;
   a.k = layer_base(*cache, cache->k, layer);
   a.v = layer_base(*cache, cache->v, layer);

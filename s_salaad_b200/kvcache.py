@@ -282,6 +282,7 @@ class PagedCache:
         [rows, heads, head_dim] (rows <= max_seqs, heads a multiple of
         kv_heads, consecutive heads share a key head), over all tokens of each
         row; ``scale`` defaults to ``head_dim ** -0.5``.  Empty rows give zeros.
+        ``out`` may be ``q`` itself, not a tensor that overlaps itself.
         Returns ``out``, or ``(out, lse)`` with the float32 log-sum-exp
         [rows, heads] (-inf for empty rows)."""
         shape, qs = self._tokens("q", q)

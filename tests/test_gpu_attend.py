@@ -109,7 +109,7 @@ def test_workspace_too_small_is_refused(cuda):
     need = lib.slr_kv_attend_workspace_size(ref, 1, 1)
     assert need > 0 and lib.slr_kv_attend_workspace_size(ref, 2, 1) == 0
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
-    for ptr, size in ((None, 0), (ws.data_ptr(), need - 1)):
+    for ptr, size in ((None, 0), (None, need), (ws.data_ptr(), need - 1)):
         rc = lib.slr_kv_attend(ref, 0, q.data_ptr(), 64, 64, out.data_ptr(), 64, 64, None, 1, 1, 1.0, ptr, size, None)
         assert rc == _lib.SLR_ERR_WORKSPACE and "workspace" in _lib.last_error()
 
@@ -360,6 +360,9 @@ def test_refusals(cuda):
         cache.attend(0, q.clone().requires_grad_())
     with torch.no_grad():
         cache.attend(0, q.clone().requires_grad_())
+    for out in (q[:1].clone().expand(2, 4, 64), q[:, :1].clone().expand(2, 4, 64)):
+        with pytest.raises(ValueError, match="overlaps itself"):
+            cache.attend(0, q, out=out)
     kv = q[:, :2]
     with pytest.raises(ValueError, match="k and v must be"):
         cache.append(0, q, q)

@@ -71,6 +71,14 @@ def test_bad_arguments():
                              None) == _lib.SLR_ERR_UNSUPPORTED
 
 
+@pytest.mark.parametrize("rows,heads,row,head", [(2, 4, 0, 64), (1, 4, 256, 0), (2, 4, 256, 63), (2, 4, 255, 64),
+                                                 (2, 2, 63, 1), (2, 4, 64, 127), (3, 4, 64, 191), (2, 4, 1 << 62, 1 << 62)])
+def test_output_that_overlaps_itself(rows, heads, row, head):
+    lib, s = _lib.load(), _cache()
+    rc = lib.slr_kv_attend(ctypes.byref(s), 0, 256, 1, 1, 256, row, head, None, rows, heads, 1.0, 256, 1 << 20, None)
+    assert rc == _lib.SLR_ERR_INVALID_ARGUMENT and "overlaps itself" in _lib.last_error()
+
+
 def test_bad_logprob_arguments():
     lib = _lib.load()
 
