@@ -32,6 +32,8 @@ def _paged_attention(module, query, key, value, attention_mask, scaling=None, **
     and value [rows, kv_heads, T, head_dim] of the T new tokens of each row."""
     if kwargs.get("sliding_window") is not None:
         raise ValueError("the paged cache has no sliding-window attention")
+    if kwargs.get("softcap") is not None or kwargs.get("s_aux") is not None:
+        raise ValueError("the paged cache has no attention with capped scores or sinks")
     cache, layer = _active.cache, module.layer_idx
     rows, heads, new, dim = query.shape
     if new == 1:
@@ -50,6 +52,9 @@ def _on_cache(model, cache: PagedCache):
     """Within the block the model's attention layers use the cache."""
     from transformers import AttentionInterface
 
+    kinds = set(getattr(model.config, "layer_types", None) or ()) - {"full_attention", "sliding_attention"}
+    if kinds:  # layers that keep a state of their own between tokens (a sliding window is refused where it is met)
+        raise ValueError(f"the paged cache holds attention layers only, the model has {sorted(kinds)}")
     AttentionInterface.register(_ATTENTION, _paged_attention)
     before = model.config._attn_implementation
     model.set_attn_implementation(_ATTENTION)

@@ -55,6 +55,20 @@ def test_request_errors():
         score(model, ids[:, :1])
 
 
+def test_other_attention_is_refused():
+    from s_salaad_b200.inference.paged import _on_cache, _paged_attention
+
+    for over in (dict(sliding_window=8), dict(softcap=30.0), dict(s_aux=torch.zeros(4))):
+        with pytest.raises(ValueError, match="the paged cache has no"):
+            _paged_attention(None, None, None, None, None, **over)
+    model = _tiny(model_type="qwen3")
+    model.config.layer_types = ["full_attention", "linear_attention"]
+    with pytest.raises(ValueError, match="linear_attention"):
+        with _on_cache(model, None):
+            pass
+    assert model.config._attn_implementation == "sdpa"
+
+
 def _tolerance(logits, dtype):
     rms, most = float(logits.pow(2).mean().sqrt()), float(logits.abs().max())
     return 1e-4 * most if dtype == F32 else 2e-2 * rms + 0.05 * most
