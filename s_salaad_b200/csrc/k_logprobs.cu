@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
     // one lane, which most batches have, then rarely costs the warp a rescaling
     if (most > st.m + 8.f) raise(most);
     if (a.top) {
-      in_group = (it & ((1 << group_log) - 1)) ? fmaxf(in_group, most) : most;
+      in_group = fmaxf((it & ((1 << group_log) - 1)) ? in_group : -INFINITY, most);  // NaN alone counts as -inf
       sh.group[it >> group_log][tid] = from_f<T>(in_group);  // exact
       const bool up = most > best;
       best = up ? most : best;
@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
         }
       }
       if (lane < k) {
-        a.top_ids[r * k + lane] = int64_t(0xffffffffu - uint32_t(list));
+        // a token whatever the row holds: callers take the ids as indexes
+        a.top_ids[r * k + lane] = min(int64_t(0xffffffffu - uint32_t(list)), a.vocab - 1);
         a.top_logprobs[r * k + lane] = logprob(value_of(list));
       }
     }
