@@ -99,16 +99,12 @@ def _decode(model, cache: PagedCache, tokens: torch.Tensor) -> torch.Tensor:
     return model(input_ids=tokens[:, None], position_ids=positions, use_cache=False).logits[:, -1]
 
 
-def _finite(logprobs: torch.Tensor) -> None:
-    if not torch.isfinite(logprobs).all():
-        raise FloatingPointError("Non-finite inference logits.")
-
-
 @torch.inference_mode()
 def generate_paged(model, input_ids: torch.Tensor, max_new_tokens: int, *, page_size: int = 16) -> torch.Tensor:
     """:func:`~s_salaad_b200.inference.generate` on a paged cache (same
     arguments, result and errors; equal greatest logits: the lowest token).
-    Logits are checked once, after the last step."""
+    Every step's logits are looked at, and an error is raised once, after the
+    last step: until then the step only notes it on the GPU."""
     from .generate import _check_request
 
     _check_request(model, input_ids, max_new_tokens)
@@ -116,17 +112,17 @@ def generate_paged(model, input_ids: torch.Tensor, max_new_tokens: int, *, page_
         return input_ids
     batch, prompt = input_ids.shape
     cache = cache_for_model(model, batch, prompt + max_new_tokens, page_size=page_size)
-    chosen, logprobs = [], []
+    chosen, finite = [], []
     with _on_cache(model, cache):
         logits = _prefill(model, cache, input_ids)
         for step in range(max_new_tokens):
             if step:
                 cache.advance(1)
                 logits = _decode(model, cache, chosen[-1])
-            best = token_logprobs(logits, top=1, entropy=False)
-            chosen.append(best.top_ids[:, 0])
-            logprobs.append(best.top_logprobs)
-    _finite(torch.cat(logprobs, dim=1))
+            finite.append(torch.isfinite(logits).all())
+            chosen.append(token_logprobs(logits, top=1, entropy=False).top_ids[:, 0])
+    if not torch.stack(finite).all():
+        raise FloatingPointError("Non-finite inference logits.")
     cache.check()
     return torch.cat([input_ids, torch.stack(chosen, dim=1)], dim=1)
 
@@ -137,7 +133,10 @@ def beam_search(model, input_ids: torch.Tensor, max_new_tokens: int, beams: int,
     """Beam search with ``beams`` (1 to 32) hypotheses per prompt of
     ``input_ids`` [batch, prompt]: (sequences [batch, beams, prompt +
     max_new_tokens], scores [batch, beams]), the score of a sequence being the
-    sum of its new tokens' log probabilities, best first."""
+    sum of its new tokens' log probabilities, best first.  -inf logits are
+    tokens of probability 0; FloatingPointError if the logits of a kept
+    hypothesis held a NaN or +inf, or fewer than ``beams`` continuations have a
+    probability above 0."""
     from .generate import _check_request
 
     _check_request(model, input_ids, max_new_tokens)
@@ -165,7 +164,8 @@ def beam_search(model, input_ids: torch.Tensor, max_new_tokens: int, beams: int,
             parents = first_row + parent
             kept = sequences.gather(1, parent[..., None].expand(batch, beams, sequences.shape[2]))
             sequences = torch.cat([kept, tokens[..., None]], dim=2)
-    _finite(scores)
+    if not torch.isfinite(scores).all():
+        raise FloatingPointError("Non-finite inference logits.")
     cache.check()
     return sequences, scores
 
