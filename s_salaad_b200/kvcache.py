@@ -306,11 +306,12 @@ class PagedCache:
                 if len(self._attend_ws) > 256:
                     self._attend_ws.clear()
                 self._attend_ws[(rows, heads)] = need
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device).data_ptr() if need else None
+            # held until the launch: a block given back before could go to another thread of this stream
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
             rc = self._lib.slr_kv_attend(
                 self._ref, layer, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
                 lse.data_ptr() if return_lse else None, rows, heads, dim ** -0.5 if scale is None else scale,
-                ws, need, _stream(self.device))
+                None if ws is None else ws.data_ptr(), need, _stream(self.device))
         finally:
             if back >= 0:
                 torch.cuda.set_device(back)
