@@ -5,7 +5,11 @@ The reference decodes greedily and recomputes the prefix every step
 sequence live in a :class:`~s_salaad_b200.kvcache.PagedCache`, the model's
 attention layers append to it and read it through an attention function
 registered with Hugging Face, and the tokens are chosen by
-:func:`~s_salaad_b200.ops.token_logprobs`; no step waits for the GPU.
+:func:`~s_salaad_b200.ops.token_logprobs`; no step waits for the GPU.  Several
+threads may generate with one model at once on one stream: each has its own
+cache, and their forwards take turns.  Other forwards of the model meanwhile use
+its own attention (they take no turn: a compressed model's layers keep one
+workspace each, so calls of one such model otherwise belong to one thread).
 
 * :func:`generate_paged` — greedy decoding (``generate(..., paged=True)``);
 * :func:`beam_search` — the ``beams`` most probable continuations found by beam
@@ -16,6 +20,7 @@ registered with Hugging Face, and the tokens are chosen by
 from __future__ import annotations
 
 import contextlib
+import sys
 import threading
 
 import torch
@@ -23,8 +28,10 @@ import torch
 from ..kvcache import PagedCache
 from ..ops import TokenLogprobs, token_logprobs
 
-_ATTENTION = "slr_paged"
-_active = threading.local()  # .cache, .cu_tokens: set while a model runs on a cache
+_active = threading.local()  # .cache, .cu_tokens, .turn: set while this thread runs a model on a cache
+_switch_lock = threading.Lock()
+_names: dict = {}  # a model's own attention -> the dispatched one
+_switched: dict = {}  # id of a config -> its _Users, while there are any
 
 
 def _paged_attention(module, query, key, value, attention_mask, scaling=None, **kwargs):
@@ -47,23 +54,72 @@ def _paged_attention(module, query, key, value, attention_mask, scaling=None, **
     return out.transpose(1, 2), None
 
 
+def _dispatched(own: str) -> str:
+    """The name of an attention that is the paged one in threads on a cache and
+    the attention ``own`` in all others."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+
+    if own in _names:
+        return _names[own]
+    name = f"slr_paged_{len(_names)}"
+
+    def attention(module, *args, **kwargs):
+        if getattr(_active, "cache", None) is not None:
+            return _paged_attention(module, *args, **kwargs)
+        known = AttentionInterface()
+        run = known[own] if own in known else sys.modules[type(module).__module__].eager_attention_forward
+        return run(module, *args, **kwargs)
+
+    def mask(*args, **kwargs):
+        known = AttentionMaskInterface()
+        if getattr(_active, "cache", None) is not None or own not in known:
+            return None
+        return known[own](*args, **kwargs)
+
+    AttentionInterface.register(name, attention)
+    AttentionMaskInterface.register(name, mask)
+    _names[own] = name
+    return name
+
+
+class _Users:
+    """The threads that have one model on caches."""
+
+    def __init__(self, model):
+        self.model, self.own, self.threads = model, model.config._attn_implementation, 0
+        # Held over a forward: compressed layers keep one workspace each, which
+        # launches of two forwards in turn would share.
+        self.turn = threading.Lock()
+
+
 @contextlib.contextmanager
 def _on_cache(model, cache: PagedCache):
-    """Within the block the model's attention layers use the cache."""
-    from transformers import AttentionInterface
-
+    """Within the block the model's attention layers use the cache, in this
+    thread: the model's attention is switched to a dispatched one by the first
+    thread that enters and back by the last that leaves."""
     kinds = set(getattr(model.config, "layer_types", None) or ()) - {"full_attention", "sliding_attention"}
     if kinds:  # layers that keep a state of their own between tokens (a sliding window is refused where it is met)
         raise ValueError(f"the paged cache holds attention layers only, the model has {sorted(kinds)}")
-    AttentionInterface.register(_ATTENTION, _paged_attention)
-    before = model.config._attn_implementation
-    model.set_attn_implementation(_ATTENTION)
-    _active.cache, _active.cu_tokens = cache, None
+    key = id(model.config)
+    with _switch_lock:
+        users = _switched.get(key)
+        if users is None:
+            users = _Users(model)
+            model.set_attn_implementation(_dispatched(users.own))
+            _switched[key] = users
+        users.threads += 1
+    outer = dict(_active.__dict__)
+    _active.cache, _active.cu_tokens, _active.turn = cache, None, users.turn
     try:
         yield
     finally:
-        model.set_attn_implementation(before)
-        del _active.cache, _active.cu_tokens
+        _active.__dict__.clear()
+        _active.__dict__.update(outer)
+        with _switch_lock:
+            users.threads -= 1
+            if not users.threads:
+                del _switched[key]
+                users.model.set_attn_implementation(users.own)
 
 
 def cache_for_model(model, max_seqs: int, max_tokens: int, *, page_size: int = 16, num_pages: int | None = None) -> PagedCache:
@@ -89,14 +145,16 @@ def _prefill(model, cache: PagedCache, input_ids: torch.Tensor) -> torch.Tensor:
     cu = torch.zeros(cache.max_seqs + 1, dtype=torch.int32, device=cache.device)
     cu[1:] = torch.cumsum(n_new, 0)
     _active.cu_tokens = cu
-    return model(input_ids=input_ids, use_cache=False, logits_to_keep=1).logits[:, -1]
+    with _active.turn:
+        return model(input_ids=input_ids, use_cache=False, logits_to_keep=1).logits[:, -1]
 
 
 def _decode(model, cache: PagedCache, tokens: torch.Tensor) -> torch.Tensor:
     """One step: tokens [rows] are the last of rows that advance() has just
     grown by one; their logits [rows, vocab]."""
     positions = (cache.lens[:tokens.shape[0]] - 1).long()[:, None]
-    return model(input_ids=tokens[:, None], position_ids=positions, use_cache=False).logits[:, -1]
+    with _active.turn:
+        return model(input_ids=tokens[:, None], position_ids=positions, use_cache=False).logits[:, -1]
 
 
 @torch.inference_mode()
