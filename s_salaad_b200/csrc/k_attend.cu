@@ -485,15 +485,13 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][0][e] += s[nt][1][e];
+        for (int e = 0; e < 4; ++e) {
+          s[nt][0][e] = __fmul_rn(s[nt][0][e] + s[nt][1][e], a.scale_log2);  // not fused, see below
+          if (valid < TT && (lane >> 2) + (e >> 1) * 8 >= valid) s[nt][0][e] = -INFINITY;
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x0 = s[nt][0][e] * a.scale_log2, x1 = s[nt][0][e + 2] * a.scale_log2;
-          if (valid < TT) {
-            if ((lane >> 2) >= valid) x0 = -INFINITY;
-            if ((lane >> 2) + 8 >= valid) x1 = -INFINITY;
-          }
-          mn[nt * 2 + e] = fmaxf(x0, x1);
+          mn[nt * 2 + e] = fmaxf(s[nt][0][e], s[nt][0][e + 2]);
           grew |= mn[nt * 2 + e] > m[nt * 2 + e] + kSlack;
         }
       }
@@ -516,6 +514,9 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
           for (int i = 0; i < DP / 4; ++i) o[nt * (DP / 4) + i] *= fac[i & 1];
         }
       }
+      // The scaled score is rounded before the reference, which is one of them,
+      // is taken from it: at scores of 10^8 the rounding of a fused product
+      // against it would be a power of two that overflows.
       // P as the sum of two 16-bit numbers (hi + lo): one alone would add an
       // error of the size of the output's own rounding.
       uint32_t hi[NT][2], lo[NT][2];
@@ -525,8 +526,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float top = m[nt * 2 + (e & 1)];
-          p[e] = ex2(fmaf(s[nt][0][e], a.scale_log2, top == -INFINITY ? 0.f : -top));
-          if (valid < TT && (lane >> 2) + (e >> 1) * 8 >= valid) p[e] = 0.f;
+          p[e] = ex2(s[nt][0][e] - (top == -INFINITY ? 0.f : top));
           l[nt * 2 + (e & 1)] += p[e];
         }
 #pragma unroll
@@ -583,12 +583,13 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       for (int g = 0; g < GT; ++g) {
         s[g] += __shfl_xor_sync(0xffffffffu, s[g], 8);
         s[g] += __shfl_xor_sync(0xffffffffu, s[g], 16);
-        grew |= t < valid && s[g] * a.scale_log2 > m[g] + kSlack;
+        s[g] = __fmul_rn(s[g], a.scale_log2);  // rounded before the reference is taken from it, as above
+        grew |= t < valid && s[g] > m[g] + kSlack;
       }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
-          float x = t < valid ? fmaxf(m[g], s[g] * a.scale_log2) : m[g];
+          float x = t < valid ? fmaxf(m[g], s[g]) : m[g];
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       }
 #pragma unroll
       for (int g = 0; g < GT; ++g) {
-        const float p = t < valid ? ex2(fmaf(s[g], a.scale_log2, m[g] == -INFINITY ? 0.f : -m[g])) : 0.f;
+        const float p = t < valid ? ex2(s[g] - (m[g] == -INFINITY ? 0.f : m[g])) : 0.f;
         if (qt == 0) {
           l[g] += p;
           pw[t * GT + g] = p;
