@@ -55,6 +55,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // many powers of two: most tiles then need one vote instead of a maximum over
 // the lanes and a rescaling.
 constexpr float kSlack = 8.f;
+// ... and lies this many below the maximum where the weights become fp16, whose
+// steps are 2^-24 at the small end: the greatest weight is 2^7 to 2^15 (fp16 ends
+// at 2^16), so small ones are held to 2^-32 of it. It cancels in the output.
+template <typename T> constexpr float kBelow = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 struct AttendK {
   const void* k;
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mn[nt * 2 + e] = fmaxf(s[nt][0][e], s[nt][0][e + 2]);
+          mn[nt * 2 + e] = fmaxf(s[nt][0][e], s[nt][0][e + 2]) - kBelow<T>;
           grew |= mn[nt * 2 + e] > m[nt * 2 + e] + kSlack;
         }
       }
@@ -527,6 +531,8 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
         for (int e = 0; e < 4; ++e) {
           const float top = m[nt * 2 + (e & 1)];
           p[e] = ex2(s[nt][0][e] - (top == -INFINITY ? 0.f : top));
+          // at scores of 10^7 the reference's own steps can put it farther below
+          if constexpr (kBelow<T> != 0.f) asm("min.NaN.f32 %0, %0, %1;" : "+f"(p[e]) : "f"(65504.f));
           l[nt * 2 + (e & 1)] += p[e];
         }
 #pragma unroll

@@ -1,11 +1,11 @@
-"""PagedCache.attend where the weights' own arithmetic shows: scores of any
-size."""
+"""PagedCache.attend where the weights' own arithmetic shows: far apart, and
+scores of any size."""
 from __future__ import annotations
 
 import pytest
 import torch
 
-from kv_model import filled_cache
+from kv_model import attention, filled_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,43 @@ def _put(cache, layer, kv, row, tokens):
     for t in range(0, n, page):
         e = min(n, t + page)
         cache.pool[layer, kv, int(cache.page_table[row, t // page]), :, :e - t] = tokens[:, t:e]
+
+
+@pytest.mark.parametrize("width,length", [(None, 300), (500, 6000)])
+@pytest.mark.parametrize("powers", [20, 24, 26])
+@pytest.mark.parametrize("first", [True, False])
+def test_one_dominating_token_in_fp16(cuda, width, length, powers, first):
+    """One token (a sink) has nearly all the weight and the value 0, the others
+    2^-20 to 2^-26 of it and large values: the output is theirs alone.
+
+    Bound: kv_model.attention's, and fp16's fixed step for small weights, which
+    are held to within 2^-32 of the greatest."""
+    dim = 64
+    cache, _, _ = filled_cache([length] * 3, kv_heads=1, dim=dim, page=16, dtype=F16, width=width)
+    q = torch.zeros(3, 2, dim, dtype=F16, device="cuda")
+    q[:, 0, 0], q[:, 1, 0] = 1.0, 0.5
+    at = 0 if first else length // 3
+    g = torch.Generator(device="cpu").manual_seed(powers)
+    keys, values = [], []
+    for r in range(3):
+        k, v = torch.zeros(1, length, dim), torch.rand(1, length, dim, generator=g) * 3e4 + 2e4
+        k[0, :, 0] = -powers * 0.6931 + torch.rand(length, generator=g) * 0.05 * r
+        k[0, at], v[0, at] = 0.0, 0.0
+        k, v = k.to(F16).cuda(), v.to(F16).cuda()
+        _put(cache, 0, 0, r, k)
+        _put(cache, 0, 1, r, v)
+        keys.append(k)
+        values.append(v)
+    got = cache.attend(0, q, scale=1.0)
+    for r in range(3):
+        o, _, tol, _ = attention(q[r], keys[r], values[r], 1.0)
+        s = torch.einsum("hd,td->ht", q[r].double(), keys[r][0].double())
+        total = torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)
+        step = 2.0 ** -32 * values[r][0].double().sum(0) / total
+        bound = tol + o.abs() * 2.0 ** -11 + step + 2.0 ** -25
+        err = (got[r].double() - o).abs()
+        assert bool((err <= bound).all()), (r, float((err / o.abs()).max()), float((bound / o.abs()).max()))
+    cache.check()
 
 
 @pytest.mark.parametrize("dtype,size", [(BF16, 1e5), (BF16, 1e18), (F16, 3e3), (F16, 6e4), (F32, 1e5), (F32, 1e18)])
@@ -48,4 +85,29 @@ def test_scores_of_any_size(cuda, dtype, size, width, sign):
     top = 0.77 * q[:, :, 0].double() * k0[:, None]
     top[3] += torch.log(torch.tensor(float(n)))
     assert bool(((lse.double() - top).abs() <= top.abs() * 2.0 ** -21).all())
+    cache.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("base", [0.0, 300.0, 2000.0, 3e4])
+@pytest.mark.parametrize("rise", [1.0, 5.0, 8.0, 13.0, 16.0])
+def test_rising_scores_far_from_zero(cuda, dtype, base, rise):
+    """Scores of about 60000 base (10^7 to 10^9) that rise by a few powers of
+    two from token to token, down to one step of fp32.  With equal values the
+    output is that value whatever the weights are: half a step of the type and
+    2^-20 for the two sums, which add the same weights."""
+    dim, n = 64, 200
+    cache, _, _ = filled_cache([n, n], kv_heads=1, dim=dim, page=16, dtype=dtype)
+    q = torch.zeros(2, 2, dim, dtype=dtype, device="cuda")
+    q[:, 0, 0], q[:, 1, 0] = 6e4, -6e4
+    q[:, :, 1] = 1.0
+    k = torch.zeros(1, n, dim)
+    k[0, :, 0] = base
+    k[0, :, 1] = torch.arange(n) * rise
+    for r in range(2):
+        _put(cache, 0, 0, r, (k if r == 0 else k.flip(1)).to(dtype).cuda())
+        _put(cache, 0, 1, r, torch.full((1, n, dim), 3.0, dtype=dtype, device="cuda"))
+    got, lse = cache.attend(0, q, scale=0.6931472, return_lse=True)
+    assert bool(((got.double() - 3.0).abs() <= 3.0 * (torch.finfo(dtype).eps / 2 + 2.0 ** -20)).all())
+    assert bool(torch.isfinite(lse).all())
     cache.check()
