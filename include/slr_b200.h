@@ -518,7 +518,7 @@ SLR_API int slr_kv_append(const slr_kv_cache* cache, int32_t layer, const void* 
  * 0, or whose scores are all -inf, gives zeros and lse = -inf; a NaN or +inf
  * score gives NaN.  Slots behind a row's length are never read into the
  * result, whatever they hold.  Products and sums are fp32; the
- * probabilities are kept to at least 16 bits (fp16: or to within 2^-32 of the
+ * probabilities are kept to at least 22 bits (fp16: or to within 2^-32 of the
  * row's greatest); out is rounded once.  The
  * result does not depend on timing, only on the inputs, the sizes of the call
  * and of the cache, and the GPU's SM count.  workspace may be NULL where

@@ -521,9 +521,14 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
       // The scaled score is rounded before the reference, which is one of them,
       // is taken from it: at scores of 10^8 the rounding of a fused product
       // against it would be a power of two that overflows.
-      // P as the sum of two 16-bit numbers (hi + lo): one alone would add an
-      // error of the size of the output's own rounding.
-      uint32_t hi[NT][2], lo[NT][2];
+      // P as a sum of 16-bit numbers, each the rounding of what the ones before
+      // leave: one alone would add an error of the size of the output's own
+      // rounding.  Two fp16 keep 22 bits, three bf16 all 24; two bf16 would keep
+      // 16, which rounds one output in 500 the other way (48 rows of up to 6007
+      // tokens: 102.4 us with two, 103.5 with three; 24 rows, groups of 16 heads
+      // of 256: 108.5, 112.6; two columns of tiles side by side gain nothing).
+      constexpr int kParts = std::is_same<T, __half>::value ? 2 : 3;
+      uint32_t part[NT][2][kParts];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float p[4];
@@ -537,10 +542,14 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t h = pair_of<T>::pack(p[j * 2], p[j * 2 + 1]);
-          const float2 back = pair_of<T>::unpack(h);
-          hi[nt][j] = transpose8(h);
-          lo[nt][j] = transpose8(pair_of<T>::pack(p[j * 2] - back.x, p[j * 2 + 1] - back.y));
+          float x0 = p[j * 2], x1 = p[j * 2 + 1];
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) {
+            const uint32_t h = pair_of<T>::pack(x0, x1);
+            const float2 back = pair_of<T>::unpack(h);
+            part[nt][j][i] = transpose8(h);
+            x0 -= back.x, x1 -= back.y;
+          }
         }
       }
       const uint32_t at = base + C::kHalf + ((lane >> 4) * 8 + r8) * C::kRow + ((((lane >> 3) & 1) ^ r8) << 4);
@@ -550,8 +559,9 @@ __global__ void __launch_bounds__(Cfg<T, DP_, GT_>::W * 32) attend_kernel(const 
         ldsm_x4_trans(at ^ (dt << 5), v[0], v[1], v[2], v[3]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma16816<T>::run(o + nt * (DP / 4) + dt * 4, v, hi[nt][0], hi[nt][1]);
-          mma16816<T>::run(o + nt * (DP / 4) + dt * 4, v, lo[nt][0], lo[nt][1]);
+#pragma unroll
+          for (int i = 0; i < kParts; ++i)
+            mma16816<T>::run(o + nt * (DP / 4) + dt * 4, v, part[nt][0][i], part[nt][1][i]);
         }
       }
     } else {

@@ -1,5 +1,5 @@
-"""PagedCache.attend where the weights' own arithmetic shows: far apart, and
-scores of any size."""
+"""PagedCache.attend where the weights' own arithmetic shows: far apart, close
+together, and scores of any size."""
 from __future__ import annotations
 
 import pytest
@@ -54,6 +54,39 @@ def test_one_dominating_token_in_fp16(cuda, width, length, powers, first):
         bound = tol + o.abs() * 2.0 ** -11 + step + 2.0 ** -25
         err = (got[r].double() - o).abs()
         assert bool((err <= bound).all()), (r, float((err / o.abs()).max()), float((bound / o.abs()).max()))
+    cache.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_weights_that_nearly_cancel(cuda, dtype):
+    """Two tokens with values 1 and -1 whose scores a and a + 2^-16 are exact in
+    fp32: the output is the difference of their weights, which 16-bit weights
+    lose.
+
+    Bound: each weight's relative error is that of the score times log2 e (two
+    roundings, |x| < 1.3: 2^-23) and of exp2 (2^-22): below 2^-21, the same for
+    the denominator; then half a step of the output."""
+    rows, dim = 128, 64
+    cache, _, _ = filled_cache([3] * rows, kv_heads=1, dim=dim, page=16, dtype=dtype)
+    a = (-torch.arange(1, rows + 1).double() / 144).to(BF16 if dtype == F32 else dtype)
+    q = torch.zeros(rows, 1, dim, dtype=dtype, device="cuda")
+    q[:, :, :2] = 1.0
+    spread, want = torch.empty(rows).double(), torch.empty(rows).double()
+    for r in range(rows):
+        k, v = torch.zeros(1, 3, dim), torch.zeros(1, 3, dim)
+        k[0, 1:, 0] = float(a[r])
+        k[0, 1, 1] = 2.0 ** -16
+        v[0, 1], v[0, 2] = 1.0, -1.0
+        _put(cache, 0, 0, r, k.to(dtype).cuda())
+        _put(cache, 0, 1, r, v.to(dtype).cuda())
+        s = torch.stack([a[r].double() * 0, a[r].double() + 2.0 ** -16, a[r].double()])
+        p = torch.softmax(s, 0)
+        want[r], spread[r] = p[1] - p[2], p[1] + p[2]
+    got = cache.attend(0, q, scale=1.0)[:, 0].double().cpu()
+    bound = want.abs() * torch.finfo(dtype).eps / 2 + spread * 2.0 ** -20
+    err = (got - want[:, None]).abs().amax(-1)
+    assert bool((err <= bound).all()), float((err / bound).max())
+    assert bool((got == got[:, :1]).all())  # all columns have the same values
     cache.check()
 
 
