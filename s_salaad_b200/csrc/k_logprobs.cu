@@ -10,7 +10,8 @@
 // a thread's batches, a block and a cluster of CTAs that share a row (few rows:
 // up to 8 CTAs per row through distributed shared memory, one launch, no
 // workspace; many rows: one CTA per row).  t is one multiply-add for two
-// elements, and -inf is raised to a finite value so that it adds 0 to u; where
+// elements (against the rounded product m·log2 e, whose error is taken back at
+// the end), and -inf is raised to a finite value so that it adds 0 to u; where
 // that is not exact (a part whose greatest logit is -inf or of the order of the
 // type's lowest or greatest value) the part is summed again element by element.
 //
@@ -239,14 +240,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   const int batches = max(1, (v1 - v0 + kThreads * kBatch - 1) / (kThreads * kBatch));
   const int group_log = 32 - __clz((batches + kGroups<T> - 1) / kGroups<T> * 2 - 1) - 1;  // batches: a power of two
   float in_group = -INFINITY;
-  auto raise = [&](float to) {
-    const float d = st.m == -INFINITY ? 0.f : log2_gap(st.m, to), f = st.m == -INFINITY ? 0.f : ex2(d);
+  // log2 e times the maximum, rounded; 0 (every 2^t is 0 then) until there is one that the product holds
+  auto base = [&] { return st.m > V::kLow ? __fmul_rn(st.m, kLog2e) : 0.f; };
+  // The sums are exact against the rounded base, so it is bases that are
+  // subtracted here, and rest() is taken back at the end of the pass: left in
+  // the sums, the rounding of a base of 10^4 would be 5e-4 of every result.
+  auto rebase = [&](float d) {
+    const float f = ex2(d);
     st.u = f * (st.u + st.s * d);
     st.s *= f;
-    st.m = to;
   };
-  // log2 e times the maximum; 0 (every 2^t is 0 then) until there is one that the product holds
-  auto base = [&] { return st.m > V::kLow ? st.m * kLog2e : 0.f; };
+  auto raise = [&](float to) {
+    const float from = base();
+    const bool any = st.m > V::kLow;  // else the sums are 0
+    st.m = to;
+    if (any) rebase(fmaxf(from - base(), -1e30f));
+  };
+  auto rest = [&] { return st.m > V::kLow ? fmaf(st.m, kLog2e, -base()) : 0.f; };
   auto batch = [&](const uint4* v, const int it) {
     typename V::Top top[kBatch];
 #pragma unroll
@@ -351,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       best_last = row.edge(tid);
     }
   }
+  rebase(-rest());
   // the triples of a warp (or of its first lanes) as one, in every lane
   auto warp_join = [&](Sums x) {
     float top = x.m;

@@ -1,4 +1,4 @@
-"""ops.token_logprobs on rows without numbers."""
+"""ops.token_logprobs on rows without numbers and on rows far from zero."""
 from __future__ import annotations
 
 import pytest
@@ -43,3 +43,29 @@ def test_best_tokens_of_rows_with_nan(cuda, dtype, vocab, copies, top):
     r = token_logprobs(kinds.cuda().repeat(copies, 1), top=top)
     assert torch.equal(r.top_ids.cpu(), want.repeat(copies, 1))
     assert bool(torch.isnan(r.entropy).all()) and bool(torch.isnan(r.top_logprobs).all())
+
+
+@pytest.mark.parametrize("dtype,shift", [(F32, 3e3), (F32, 1e6), (F32, -1e6), (F16, 3e4)])
+@pytest.mark.parametrize("rows,vocab", [(5, 1001), (700, 1001), (3, 32000)])
+def test_logits_far_from_zero(cuda, dtype, shift, rows, vocab):
+    """A number added to all logits of a row changes nothing: the error goes by
+    the distance from the greatest logit, not by the logits' own size.
+
+    Bounds: the sums' relative error (2^-20 + vocab 2^-24) and the rounding of
+    x - max, of its product with log2 e and of the last subtraction (2^-22 of
+    |x - max| + log vocab)."""
+    g = torch.Generator(device="cpu").manual_seed(int(abs(shift)) + rows)
+    x = (torch.randn(rows, vocab, generator=g) * 2.5 + shift).to(dtype).cuda()
+    t = torch.randint(0, vocab, (rows,), generator=g).cuda()
+    r = token_logprobs(x, t, top=5)
+    d = x.double()
+    d = d - d.amax(-1, keepdim=True)
+    logp = d - torch.logsumexp(d, -1, keepdim=True)
+    rel = 2.0 ** -20 + vocab * 2.0 ** -24
+    tol = rel + 2.0 ** -22 * (d.abs() + torch.log(torch.tensor(float(vocab))))
+    err = (r.logprob.double()[:, None] - logp.gather(1, t[:, None])).abs()
+    assert bool((err <= tol.gather(1, t[:, None])).all()), float(err.max())
+    err = (r.top_logprobs.double() - logp.gather(1, r.top_ids)).abs()
+    assert bool((err <= tol.gather(1, r.top_ids)).all()), float(err.max())
+    ent, mean = -(logp.exp() * logp).sum(-1), (logp.exp() * d.abs()).sum(-1)
+    assert bool(((r.entropy.double() - ent).abs() <= rel * (2 * mean + 1) + ent * 2.0 ** -22).all())
