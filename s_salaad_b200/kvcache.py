@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _DeviceGuard, _no_graph, _require_cuda, _stream, _switch, slr_dtype
@@ -76,6 +77,7 @@ class PagedCache:
                 raise ValueError(f"pool must be {shape}, got {tuple(pool.shape)}")
             if head_dim > 1 and pool.stride(5) != 1:
                 raise ValueError("pool must have unit stride in the last dimension")
+            _no_graph("PagedCache (pool)", pool)
         if state is not None:
             _require_cuda("state", state)
             if state.dtype != torch.int32:
@@ -248,7 +250,7 @@ class PagedCache:
             raise ValueError(f"{name} must be [tokens, heads, {self.head_dim}], got {tuple(shape)}")
         if stride[2] != 1:
             raise ValueError(f"{name} must have unit stride in the last dimension")
-        if t.requires_grad:
+        if t.requires_grad or forward_ad._current_level >= 0:  # (calls of a few microseconds)
             _no_graph(f"PagedCache ({name})", t)
         return shape, stride
 

@@ -21,6 +21,7 @@ from typing import NamedTuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -680,11 +681,14 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor | None  # [..., top]
 
 
-def _no_graph(name: str, *tensors: torch.Tensor) -> None:
-    """The library's operators compute values only: refuse inputs that a
-    gradient would be expected of, instead of dropping it."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_graph(name: str, t: torch.Tensor) -> None:
+    """The library's operators compute values only: refuse an input that a
+    gradient, or within forward_ad.dual_level() a tangent, would be expected of,
+    instead of dropping it."""
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} has no backward pass; call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has no forward-mode derivative; call it on the primal (unpack_dual)")
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top: int = 0,
@@ -717,8 +721,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
             raise ValueError(f"targets must be {tuple(shape)} on {dev}")
         if not targets.is_contiguous():
             targets = targets.contiguous()
-    if logits.requires_grad:
-        _no_graph("token_logprobs", logits)
+    _no_graph("token_logprobs", logits)
     x = logits if len(full) == 2 else logits.reshape(-1, vocab)
     rows = x.shape[0]
     stride, unit = x.stride()

@@ -4,7 +4,9 @@ from __future__ import annotations
 
 import weakref
 
+import pytest
 import torch
+from torch.autograd import forward_ad
 
 from s_salaad_b200 import _lib, kvcache
 from s_salaad_b200.kvcache import PagedCache
@@ -49,3 +51,52 @@ def test_the_workspace_lives_until_the_call_returns(monkeypatch):
     monkeypatch.setattr(torch, "empty", recording)
     _host_cache(Lib).attend(0, torch.zeros(3, 4, 64, dtype=torch.bfloat16))
     assert seen == [(4096, True)]
+
+
+class _Accepts:
+    """A library that takes every call."""
+
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+def test_gradients_and_tangents_are_refused(monkeypatch):
+    """An input that a derivative would be expected of, in either mode, is an
+    error and not a result without one."""
+    monkeypatch.setattr(kvcache, "_switch", lambda index: -1)
+    monkeypatch.setattr(kvcache, "_stream", lambda device: 0)
+    cache = _host_cache(_Accepts())
+    q, kv = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        dq, dkv = forward_ad.make_dual(q, q), forward_ad.make_dual(kv, kv)
+        for call in (lambda: cache.attend(0, dq), lambda: cache.attend(0, q, out=dq),
+                     lambda: cache.append(0, dkv, kv), lambda: cache.append(0, kv, dkv),
+                     lambda: cache.append(0, dkv[:, :, :], kv)):
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                call()
+        cache.attend(0, forward_ad.unpack_dual(dq).primal)
+        cache.attend(0, q)
+        cache.append(0, kv, kv)
+        with torch.inference_mode():  # no derivatives here
+            cache.attend(0, dq)
+    for call in (lambda: cache.attend(0, q.clone().requires_grad_()), lambda: cache.append(0, kv, kv.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+@pytest.mark.gpu
+def test_tangents_and_a_pool_with_gradients_are_refused(cuda):
+    from s_salaad_b200.ops import token_logprobs
+
+    x = torch.randn(3, 50, device=cuda)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="no forward-mode derivative"):
+            token_logprobs(forward_ad.make_dual(x, x), top=2)
+        token_logprobs(x, top=2)
+    pool = torch.zeros(1, 2, 4, 1, 16, 64, dtype=torch.bfloat16, device=cuda)
+    kw = dict(num_layers=1, num_pages=4, kv_heads=1, head_dim=64, max_seqs=1, max_pages=1)
+    with pytest.raises(ValueError, match="no backward"):
+        PagedCache(**kw, pool=pool.clone().requires_grad_())
+    PagedCache(**kw, pool=pool)
