@@ -238,7 +238,7 @@ def score(model, input_ids: torch.Tensor, *, top: int = 0, ignore_id: int | None
         raise ValueError("Expected a batch of at least two input token IDs each.")
     logits = model(input_ids=input_ids, use_cache=False).logits
     # the last position predicts nothing: scoring it too keeps the rows packed
-    targets = torch.full_like(input_ids, -100)
+    targets = torch.full_like(input_ids, -100, dtype=torch.int64)
     targets[:, :-1] = input_ids[:, 1:]
     if ignore_id is not None:
         targets.masked_fill_(targets == ignore_id, -100)

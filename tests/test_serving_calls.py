@@ -100,3 +100,24 @@ def test_tangents_and_a_pool_with_gradients_are_refused(cuda):
     with pytest.raises(ValueError, match="no backward"):
         PagedCache(**kw, pool=pool.clone().requires_grad_())
     PagedCache(**kw, pool=pool)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_score_takes_the_ids_that_the_model_takes(monkeypatch, dtype):
+    """Embeddings index with int32 too; the targets are the next ids either way."""
+    from types import SimpleNamespace
+
+    from s_salaad_b200.inference import paged
+
+    seen = {}
+
+    def scores(logits, targets, *, top):
+        seen["targets"] = targets
+        return paged.TokenLogprobs(torch.zeros(2, 4), torch.zeros(2, 4), None, None)
+
+    monkeypatch.setattr(paged, "token_logprobs", scores)
+    ids = torch.tensor([[1, 2, 3, 0], [4, 5, 6, 7]], dtype=dtype)
+    r = paged.score(lambda **kw: SimpleNamespace(logits=torch.zeros(2, 4, 9)), ids, ignore_id=0)
+    assert r.logprob.shape == (2, 3)
+    assert seen["targets"].dtype == torch.int64
+    assert seen["targets"].tolist() == [[2, 3, -100, -100], [5, 6, 7, -100]]
