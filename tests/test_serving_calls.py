@@ -121,3 +121,18 @@ def test_score_takes_the_ids_that_the_model_takes(monkeypatch, dtype):
     assert r.logprob.shape == (2, 3)
     assert seen["targets"].dtype == torch.int64
     assert seen["targets"].tolist() == [[2, 3, -100, -100], [5, 6, 7, -100]]
+
+
+def test_cache_for_model_takes_the_number_of_pages_as_given(monkeypatch):
+    """0 pages are refused (by PagedCache), not replaced by the default."""
+    from types import SimpleNamespace
+
+    from s_salaad_b200.inference import paged
+
+    made = []
+    monkeypatch.setattr(paged, "PagedCache", lambda **kw: made.append(kw["num_pages"]))
+    model = SimpleNamespace(config=SimpleNamespace(hidden_size=64, num_attention_heads=4, num_hidden_layers=1),
+                            parameters=lambda: iter([torch.zeros(1)]))
+    for pages in (None, 0, 7):
+        paged.cache_for_model(model, 3, 40, num_pages=pages)
+    assert made == [3 * (3 + 1), 0, 7]
