@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import test_gpu_attend as attend_tests
 from kv_model import attention, filled_cache
 
 pytestmark = pytest.mark.gpu
@@ -144,3 +145,15 @@ def test_rising_scores_far_from_zero(cuda, dtype, base, rise):
     assert bool(((got.double() - 3.0).abs() <= 3.0 * (torch.finfo(dtype).eps / 2 + 2.0 ** -20)).all())
     assert bool(torch.isfinite(lse).all())
     cache.check()
+
+
+def test_scales_growing_scores_and_infinities_in_fp16(cuda):
+    """What test_gpu_attend has in bf16 and fp32, with its bounds."""
+    attend_tests.test_growing_scores(cuda, F16)
+    attend_tests.test_infinities_and_nan(cuda, F16)
+    for scale in (-0.3, 0.0, 3.0):
+        attend_tests.test_scales(cuda, scale, F16)
+    attend_tests.test_one_q_for_all_rows_and_heads(cuda, F16)
+    attend_tests.test_many_ragged_rows(cuda, F16)
+    for width in (None, 30, 900, 5000):
+        attend_tests.test_few_short_rows(cuda, F16, 256, 20, 1, width)
