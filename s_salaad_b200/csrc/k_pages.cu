@@ -506,15 +506,10 @@ constexpr int kCopyUnroll = 4;
 // 24: 258, 64: 252).  Copies that are mostly empty keep to one wave of 8.
 constexpr int kManyCtas = 64;
 
-template <int V> struct vec_of;
-template <> struct vec_of<16> { using type = uint4; };
-template <> struct vec_of<4> { using type = uint32_t; };
-
 // Pages src[i] -> dst[i] of every plane.  An item is a piece of one page of
 // one plane; CTAs take the items in turn.
-template <int V>
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyK a) {
-  using Vec = typename vec_of<V>::type;
+  using Vec = uint4;  // a page's bytes are a multiple of 16
   pdl_wait_primary();
   const int tid = threadIdx.x;
   if (a.table) {
@@ -528,7 +523,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyK a) {
     }
   }
   const int n = a.count ? *a.count : a.n;
-  constexpr int64_t kPiece = int64_t(kCopyThreads) * kCopyUnroll * V;
+  constexpr int64_t kPiece = int64_t(kCopyThreads) * kCopyUnroll * sizeof(Vec);
   const int64_t pieces = (a.page_bytes + kPiece - 1) / kPiece;
   const int64_t per_pair = pieces * a.planes;
   int last = -1;
@@ -557,12 +552,12 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const CopyK a) {
     Vec x[kCopyUnroll];
 #pragma unroll
     for (int i = 0; i < kCopyUnroll; ++i) {
-      const int64_t at = (int64_t(i) * kCopyThreads + tid) * V;
+      const int64_t at = (int64_t(i) * kCopyThreads + tid) * int64_t(sizeof(Vec));
       if (at < left) x[i] = *reinterpret_cast<const Vec*>(from + at);
     }
 #pragma unroll
     for (int i = 0; i < kCopyUnroll; ++i) {
-      const int64_t at = (int64_t(i) * kCopyThreads + tid) * V;
+      const int64_t at = (int64_t(i) * kCopyThreads + tid) * int64_t(sizeof(Vec));
       if (at < left) *reinterpret_cast<Vec*>(to + at) = x[i];
     }
   }
@@ -697,9 +692,9 @@ int copy_launch(const PagesArgs& p, CopyK c, int64_t most_pairs, int64_t ctas, c
   c.page_bytes = p.page_bytes;
   c.planes = 2 * p.layers;
   c.num_pages = p.num_pages;
-  const int64_t pieces = ceil_div(p.page_bytes, int64_t(kCopyThreads) * kCopyUnroll * 16);
+  const int64_t pieces = ceil_div(p.page_bytes, int64_t(kCopyThreads) * kCopyUnroll * int64_t(sizeof(uint4)));
   const int64_t items = std::max<int64_t>(1, pieces * c.planes * most_pairs);
-  return launch_after(copy_kernel<16>, dim3(unsigned(std::min(items, ctas))), kCopyThreads, 0, s, c);
+  return launch_after(copy_kernel, dim3(unsigned(std::min(items, ctas))), kCopyThreads, 0, s, c);
 }
 
 }  // namespace
