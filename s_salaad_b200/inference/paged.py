@@ -88,8 +88,8 @@ class _Users:
     def __init__(self, model):
         self.model, self.own, self.threads = model, model.config._attn_implementation, 0
         # Held over a forward: compressed layers keep one workspace each, which
-        # launches of two forwards in turn would share.
-        self.turn = threading.Lock()
+        # launches of two forwards in turn would share.  (A hook may generate, too.)
+        self.turn = threading.RLock()
 
 
 @contextlib.contextmanager

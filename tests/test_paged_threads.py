@@ -146,6 +146,42 @@ def test_an_error_in_one_thread_leaves_the_others(monkeypatch):
     assert model.config._attn_implementation == "sdpa"
 
 
+def test_a_forward_hook_that_generates():
+    """A generation inside a forward on a cache: the inner one has its own
+    cache, and the outer one goes on with its own."""
+    model = _model("sdpa")
+    ids, other = torch.arange(10).view(2, 5), torch.arange(50, 58).view(2, 4)
+    got = {}
+
+    def inner(module, args):
+        if "inner" not in got:
+            got["inner"] = None
+            cache = HostCache(2)
+            with _on_cache(model, cache):
+                got["inner"] = _prefill(model, cache, other)
+
+    with torch.inference_mode():
+        want, want_inner = (model(input_ids=i, use_cache=False).logits[:, -1] for i in (ids, other))
+        hook = model.model.layers[1].register_forward_pre_hook(inner)
+        done = threading.Event()
+
+        def outer():
+            with torch.inference_mode():
+                cache = HostCache(2)
+                with _on_cache(model, cache):
+                    _prefill(model, cache, ids[:, :4])
+                    cache.advance(1)
+                    got["outer"] = _decode(model, cache, ids[:, 4])
+            done.set()
+
+        threading.Thread(target=outer, daemon=True).start()
+        assert done.wait(60)
+    hook.remove()
+    for a, b in ((got["inner"], want_inner), (got["outer"], want)):
+        assert bool(((a - b).abs() <= 1e-4 * b.abs().max()).all())
+    assert model.config._attn_implementation == "sdpa"
+
+
 @pytest.mark.gpu
 def test_threads_with_a_compressed_model(cuda, tmp_path):
     """Each thread gets what it gets alone, bit by bit (the layers' kernels do
