@@ -130,7 +130,9 @@ def cache_for_model(model, max_seqs: int, max_tokens: int, *, page_size: int = 1
     dim = getattr(c, "head_dim", None) or c.hidden_size // c.num_attention_heads
     width = -(-max_tokens // page_size)
     p = next(model.parameters())
-    return PagedCache(num_layers=c.num_hidden_layers, num_pages=max_seqs * (width + 1) if num_pages is None else num_pages,
+    if num_pages is None:
+        num_pages = max_seqs * (width + 1)
+    return PagedCache(num_layers=c.num_hidden_layers, num_pages=num_pages,
                       kv_heads=getattr(c, "num_key_value_heads", None) or c.num_attention_heads, head_dim=dim,
                       page_size=page_size, max_seqs=max_seqs, max_pages=width, dtype=p.dtype, device=p.device)
 
