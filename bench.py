@@ -20,7 +20,8 @@ block-row sharded over the ranks and y is all-gathered (NCCL), so the total
 work is fixed (strong scaling).  `--impl reference` times the reference's
 CPU implementation of the path (its AVX2 BSR kernel, compiled from the
 reference sources into oracle/_ref, plus the low-rank F.linear calls and the
-bias, in fp32) on this host's cores over the same token batch.
+bias, in fp32) on this host's cores over the same token batch; where that
+kernel is not built it prints {"impl": "reference", "unavailable": why}.
 """
 from __future__ import annotations
 
@@ -210,8 +211,10 @@ class ClockSampler:
 
 def cpu_reference_run(specs, T_sample: int, steps: int, warmup: int, budget_s: float | None):
     """Time the reference CPU path (AVX2 kernel from oracle/_ref + MKL
-    F.linear + bias, fp32) on T_sample tokens through the layer set.
-    Returns (seconds per sample, kind, cores, CPU model name)."""
+    F.linear + bias, fp32) on T_sample tokens through the layer set.  Where
+    that kernel is not built, the plain C port is timed, on as many of the
+    tokens as four passes fit the budget with (it is 20 times slower).
+    Returns (seconds per sample, tokens, kind, cores, CPU model name)."""
     sys.path.insert(0, str(REPO / "oracle"))
     import slr_oracle  # noqa: E402  (CPU baseline leg)
 
@@ -222,13 +225,12 @@ def cpu_reference_run(specs, T_sample: int, steps: int, warmup: int, budget_s: f
     kind = "reference" if mod is not None else "port"
     from s_salaad_b200 import workloads
 
-    layers = []
-    for s in specs:
-        t = s.tensors("cpu", torch.float32)
-        x = workloads.tokens(T_sample, s.in_features, seed=7)
-        layers.append((t, x))
+    tensors = [s.tensors("cpu", torch.float32) for s in specs]
 
-    def one():
+    def batches(n):
+        return [(t, workloads.tokens(n, s.in_features, seed=7)) for s, t in zip(specs, tensors)]
+
+    def one(layers):
         for t, x in layers:
             if mod is not None:
                 slr_oracle.lrs_forward_f32_ref_kernel(x, t["A"], t["B"], t["S_crow"], t["S_col"], t["S_values"],
@@ -237,13 +239,21 @@ def cpu_reference_run(specs, T_sample: int, steps: int, warmup: int, budget_s: f
                 slr_oracle.lrs_forward_f32(x, t["A"], t["B"], t["S_crow"], t["S_col"], t["S_values"],
                                            t["S_active_rows"], t["bias"])
 
+    if mod is None and budget_s is not None:
+        few = batches(min(T_sample, 4))
+        one(few)
+        t0 = time.perf_counter()
+        one(few)
+        per_token = (time.perf_counter() - t0) / len(few[0][1])
+        T_sample = max(1, min(T_sample, int(budget_s / (4 * per_token))))
+    layers = batches(T_sample)
     for _ in range(max(warmup, 1)):
-        one()
+        one(layers)
     times = []
     t_end = None if budget_s is None else time.perf_counter() + budget_s
     while True:
         t0 = time.perf_counter()
-        one()
+        one(layers)
         times.append(time.perf_counter() - t0)
         if budget_s is None and len(times) >= steps:
             break
@@ -251,7 +261,7 @@ def cpu_reference_run(specs, T_sample: int, steps: int, warmup: int, budget_s: f
             break
     if kind == "port":
         cores = 1
-    return times, kind, cores, cpu_model
+    return times, T_sample, kind, cores, cpu_model
 
 
 def cpu_model_name() -> str:
@@ -563,7 +573,13 @@ def main() -> None:
     if args.impl == "reference":
         if rank != 0:
             return
-        times, kind, cores, model = cpu_reference_run(specs, T_sample, args.steps, args.warmup, None)
+        sys.path.insert(0, str(REPO / "oracle"))
+        import slr_oracle
+
+        if slr_oracle.ref_avx2_module() is None:
+            emit({"impl": "reference", "unavailable": "the reference's CPU kernel is not built (no reference sources here)"})
+            return
+        times, _, kind, cores, model = cpu_reference_run(specs, T_sample, args.steps, args.warmup, None)
         tok_s = T_sample * len(times) / sum(times)
         line = {"metric": METRIC, "impl": "reference", "value": tok_s, "unit": "tokens/s", "n_gpus": world,
                 "steps": len(times), "warmup": args.warmup, "ms_per_step": 1e3 * statistics.mean(times),
@@ -1107,11 +1123,12 @@ def main() -> None:
     # ------------------------------------------------------- CPU baseline
     cpu = None
     if world == 1 and rank == 0 and not args.no_cpu_baseline:
-        times, kind, cores, model = cpu_reference_run(specs, T_sample, 0, 1, args.cpu_budget_s)
-        cpu = {"value": T_sample * len(times) / sum(times), "unit": "tokens/s", "cores": cores, "kind": kind,
+        times, n_cpu, kind, cores, model = cpu_reference_run(specs, T_sample, 0, 1, args.cpu_budget_s)
+        what = "reference AVX2 BSR kernel + MKL low-rank + bias" if kind == "reference" else "plain C port, one core"
+        cpu = {"value": n_cpu * len(times) / sum(times), "unit": "tokens/s", "cores": cores, "kind": kind,
                "cpu_model": model,
-               "sample": f"{T_sample} of {T} tokens x {len(times)} reps through all {len(specs)} projections, "
-                         f"fp32 (reference AVX2 BSR kernel + MKL low-rank + bias)"}
+               "sample": f"{n_cpu} of {T} tokens x {len(times)} reps through all {len(specs)} projections, "
+                         f"fp32 ({what})"}
 
     if rank == 0:
         all_flops = sum(s.flops_per_token() for s in specs) * T
